@@ -50,6 +50,10 @@ class FcLlamaWeights(C.Structure):
                 ("output_q8", C.c_void_p), ("rope_freqs", C.c_void_p)]
 
 
+class FcRowSampling(C.Structure):
+    _fields_ = [("temperature", C.c_float), ("top_k", C.c_int32), ("top_p", C.c_float), ("min_p", C.c_float)]
+
+
 FC_ROPE_NORM, FC_ROPE_NEOX = 0, 1
 FC_Q_INT8, FC_Q_INT4 = 0, 1
 
@@ -147,6 +151,14 @@ SIGNATURES = {
     "fc_rowq_free": (None, [C.c_void_p]),
     "fc_rowq_linear": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int]),
     "fc_rowq_linear_dev": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p]),
+    "fc_kv4_create": (C.c_int, [C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.POINTER(C.c_void_p)]),
+    "fc_kv4_free": (None, [C.c_void_p]),
+    "fc_kv4_append_dev": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p]),
+    "fc_kv4_attend_dev": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_float,
+                                    C.c_void_p, C.c_void_p, C.c_int, C.c_void_p]),
+    "fc_kv4_read_dev": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p]),
+    "fc_kv4_evict_dev": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
+    "fc_sample_rows_dev": (C.c_int, [C.c_int, C.c_void_p, C.c_int64, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
     "fc_take_launch_count": (C.c_int64, []),
     "fc_last_decode_ms": (C.c_float, [C.c_void_p]),
     "fc_last_score_ms": (C.c_float, [C.c_void_p]),

@@ -1,0 +1,23 @@
+// Launchers of the 4-bit cache's kernels (kv4.cu, kv4_attend.cu).
+#pragma once
+#include <algorithm>
+
+#include "kv4.cuh"
+
+namespace fc {
+
+struct Kv4Attend {
+    const float *q, *k, *v;      // k, v: the call's new rows, or null
+    float* out;
+    int ldq, ldkv, ldo;
+    int group;                   // query heads a key / value head
+    float scale;
+    const int* lens;             // positions before the call (k, v given) or with the call's rows
+    float* mass;                 // [n_seq][n_kv][cap] or null
+};
+
+int make_device(int device);
+int launch_kv4_append(const Kv4& c, const float* k, const float* v, int ldkv, const KvRows& rows, int max_rows, const int* lens, cudaStream_t st);
+int launch_kv4_attend(const Kv4& c, const Kv4Attend& a, const KvRows& rows, int max_rows, int device, cudaStream_t st);
+
+}  // namespace fc

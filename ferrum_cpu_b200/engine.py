@@ -50,6 +50,14 @@ def sample_logits(logits, rng_state, params, recent=(), device=0):
     return tok.value, state.value
 
 
+def sample_rows_dev(logits_ptr, ld, n_rows, vocab, params_ptr, u_ptr, token_ptr, prob_ptr=None, device=0, stream=None):
+    """One draw from each row of logits on the device (temperature, top-k, top-p, min-p), with random numbers u that the caller
+    gives; params_ptr: FcRowSampling [n_rows]."""
+    rc = _lib.lib().fc_sample_rows_dev(device, logits_ptr, ld, n_rows, vocab, params_ptr, u_ptr, token_ptr, prob_ptr, stream)
+    if rc:
+        check(rc)
+
+
 def gguf_probe(path, row_perm=None):
     """Dimensions of a gpt2-architecture GGUF file; validates it without a GPU."""
     perm = None if row_perm is None else np.ascontiguousarray(row_perm, dtype=np.int32)

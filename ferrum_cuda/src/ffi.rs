@@ -68,6 +68,9 @@ pub struct fc_layer_stats { pub min: f32, pub max: f32, pub mean: f32, pub nan_c
 #[derive(Clone, Copy, Debug)]
 pub struct fc_sampling { pub temperature: f32, pub top_k: i32, pub top_p: f32, pub repetition_penalty: f32 }
 #[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct fc_row_sampling { pub temperature: f32, pub top_k: i32, pub top_p: f32, pub min_p: f32 }
+#[repr(C)]
 #[derive(Clone, Copy, Debug, Default)]
 pub struct fc_llama_config {
     pub vocab: i32, pub d_model: i32, pub n_layer: i32, pub n_head: i32, pub n_kv_head: i32, pub head_dim: i32, pub d_ff: i32,
@@ -96,6 +99,7 @@ pub enum fc_ggml_weight {}
 pub enum fc_llama {}
 pub enum fc_llama_cache {}
 pub enum fc_rowq {}
+pub enum fc_kv4 {}
 
 #[link(name = "ferrum_cuda")]
 extern "C" {
@@ -178,6 +182,13 @@ extern "C" {
     pub fn fc_rowq_free(w: *mut fc_rowq);
     pub fn fc_rowq_linear(w: *const fc_rowq, x: *const f32, bias: *const f32, y: *mut f32, M: c_int) -> c_int;
     pub fn fc_rowq_linear_dev(w: *const fc_rowq, x_dev: *const f32, bias_dev: *const f32, y_dev: *mut f32, M: c_int, stream: *mut c_void) -> c_int;
+    pub fn fc_kv4_create(device: c_int, n_seq: c_int, n_kv_head: c_int, head_dim: c_int, capacity: c_int, out: *mut *mut fc_kv4) -> c_int;
+    pub fn fc_kv4_free(c: *mut fc_kv4);
+    pub fn fc_kv4_append_dev(c: *mut fc_kv4, k: *const f32, v: *const f32, ldkv: c_int, rows: *const i32, lens: *const i32, stream: *mut c_void) -> c_int;
+    pub fn fc_kv4_attend_dev(c: *mut fc_kv4, q: *const f32, ldq: c_int, n_head: c_int, k: *const f32, v: *const f32, ldkv: c_int, rows: *const i32, lens: *const i32, scale: f32, mass: *mut f32, out: *mut f32, ldo: c_int, stream: *mut c_void) -> c_int;
+    pub fn fc_kv4_read_dev(c: *const fc_kv4, from: *const i32, n: c_int, k: *mut f32, v: *mut f32, stream: *mut c_void) -> c_int;
+    pub fn fc_kv4_evict_dev(src: *const fc_kv4, dst: *mut fc_kv4, lens: *const i32, lens_out: *mut i32, budget: c_int, recent: c_int, mass: *const f32, mass_out: *mut f32, kept: *mut i32, stream: *mut c_void) -> c_int;
+    pub fn fc_sample_rows_dev(device: c_int, logits: *const f32, ld: i64, n_rows: c_int, vocab: c_int, params: *const fc_row_sampling, u: *const f32, token: *mut i32, prob: *mut f32, stream: *mut c_void) -> c_int;
     pub fn fc_take_launch_count() -> i64;
     pub fn fc_last_decode_ms(s: *const fc_stream) -> f32;
     pub fn fc_last_score_ms(m: *const fc_model) -> f32;

@@ -506,6 +506,62 @@ int fc_rowq_linear(const fc_rowq* w, const float* x, const float* bias, float* y
  * whose scratch grows in the handle: one stream at a time, and a call of that size before a capture. */
 int fc_rowq_linear_dev(const fc_rowq* w, const float* x_dev, const float* bias_dev, float* y_dev, int M, void* stream);
 
+/* ---- a key / value cache of 4-bit levels, and draws from rows of logits ------------ */
+/* What a serving loop keeps between tokens at 4.5 bits a value, for n_seq sequences (256 at most) of `capacity` positions: rows of
+ * head_dim values (a multiple of 32, at most 256) a key / value head. A row is cut into blocks of 32 with an f16 scale
+ * d = f16(m / -8), m the block's value of largest magnitude (the positive one where two tie; |d| at most 65504), and levels
+ * clamp(rint(x / d), -8, 7): what is cached is d * level. NaN counts as 0.
+ * The calls below work on device pointers and return before their kernels run, in the order of `stream` (a cudaStream_t, or
+ * NULL); none waits, all can be captured into a graph, where the lengths are read anew at every replay. The lengths
+ * themselves belong to the caller: lens [n_seq] on the device, the positions of each sequence that hold something. A caller
+ * that sets one back has dropped what lay behind it. Calls on one cache that may overlap are the caller's to order, unless
+ * all of them only read. Handles are created and freed as weights are. */
+typedef struct fc_kv4 fc_kv4;
+int fc_kv4_create(int device, int n_seq, int n_kv_head, int head_dim, int capacity, fc_kv4** out);
+void fc_kv4_free(fc_kv4* c);
+/* New rows of keys and values: k, v [sum of rows][n_kv_head * head_dim], ldkv floats apart (a multiple of 4; both 16-byte aligned). `rows`
+ * [n_seq] on the HOST says how many each sequence brings (0: none); NULL: one each. Row i of sequence s goes to position
+ * lens[s] + i; lens itself is not changed. A sequence whose length is negative or whose rows do not fit is left alone. */
+int fc_kv4_append_dev(fc_kv4* c, const float* k, const float* v, int ldkv, const int32_t* rows, const int32_t* lens, void* stream);
+/* Causal attention over the cache: out = softmax(scale * q K^T) V for query rows q [sum of rows][n_head * head_dim], n_head a
+ * multiple of n_kv_head (heads of a group lie side by side). scale 0 stands for 1 / sqrt(head_dim).
+ * With k and v the rows first go into the cache as fc_kv4_append_dev has it, and row i attends to the positions
+ * 0 .. lens[s] + i; without them (both NULL) the rows are the last `rows[s]` of the lens[s] positions that are cached: row i attends to
+ * 0 .. lens[s] - rows[s] + i, and a row that sees nothing is zeros.
+ * mass (may be NULL) [n_seq][n_kv_head][capacity]: the weights that a position receives in this call, over the rows and the heads
+ * that share it, are added to it; a position that the call brings starts from nothing.
+ * Sums and statistics are held in f32 and the levels are exact: the result is that of f32 arithmetic on the cached values, bitwise
+ * repeatable. Pointers 16-byte aligned, ldq, ldkv, ldo multiples of 4; out overlaps nothing else. The rows of a sequence whose
+ * length is negative or whose rows do not fit are NaN, and its cache and mass are left alone. */
+int fc_kv4_attend_dev(fc_kv4* c, const float* q, int ldq, int n_head, const float* k, const float* v, int ldkv, const int32_t* rows,
+                      const int32_t* lens, float scale, float* mass, float* out, int ldo, void* stream);
+/* What positions from[s] .. from[s] + n - 1 of every sequence stand for (from: device [n_seq], NULL: 0): k, v [n_seq][n][n_kv_head][head_dim].
+ * Positions outside the cache are zeros. */
+int fc_kv4_read_dev(const fc_kv4* c, const int32_t* from, int n, float* k, float* v, void* stream);
+/* Eviction by accumulated weight, a key / value head at a time: of the lens[s] positions the last `recent` and the heaviest
+ * others (by mass [n_seq][n_kv_head][capacity of src]; the lower position where two weigh the same, NaN the least), `budget` in all, go to
+ * `dst`, another cache of the same sequences and heads, in their order; a sequence of at most `budget` positions goes whole.
+ * lens_out [n_seq] (not lens): what is left. mass_out [n_seq][n_kv_head][capacity of dst] (may be NULL): their weights. kept
+ * [n_seq][n_kv_head][budget] (may be NULL): their positions in src, -1 behind the last. dst, mass_out behind what is left stay as they were. */
+int fc_kv4_evict_dev(const fc_kv4* src, fc_kv4* dst, const int32_t* lens, int32_t* lens_out, int budget, int recent, const float* mass,
+                     float* mass_out, int32_t* kept, void* stream);
+
+/* The parameters of one row's draw. temperature <= 0 (or NaN): the first of the largest logits; others count as 0.01 at
+ * least. top_k <= 0, top_p >= 1, min_p <= 0 (or NaN): no such filter. */
+typedef struct {
+    float temperature;
+    int32_t top_k;
+    float top_p, min_p;
+} fc_row_sampling;
+/* One draw from each of n_rows rows of `vocab` logits (2^24 at most), ld floats apart, with given random numbers u [n_rows] in [0, 1).
+ * w = exp((l - max) / temperature) in 64 bits. As in fc_sample_logits, all of a tie at a cut stays: ids that are not below the top_k-th
+ * largest logit, nor below the largest logit down to which the mass reaches top_p of the whole row; and w >= min_p. Of what
+ * stays, weights under 2^-40 are nothing. The token is the first id, in index order, at which the running mass reaches u
+ * times the whole; prob (may be NULL) its share of the whole. NaN logits are forbidden ids, as -inf; a row
+ * without any other has token -1 and prob 0. All pointers on the device, params 16-byte aligned; asynchronous on `stream`, nothing is allocated. */
+int fc_sample_rows_dev(int device, const float* logits, int64_t ld, int n_rows, int vocab, const fc_row_sampling* params, const float* u,
+                       int32_t* token, float* prob, void* stream);
+
 /* ---- introspection used by the benchmark ----------------------------------------- */
 /* Kernel launches issued by this library on the calling thread since the last call
  * (returns the count and resets it). */
