@@ -3,59 +3,38 @@
 #include <climits>
 #include <cmath>
 
-#include "kv4_ops.cuh"
+#include "kv4_frag.cuh"
 
 namespace fc {
 
 namespace {
 
-// One block of 32 values, one a lane: its scale and this lane's level plus 8. The quotient of two f32 never rounds onto a tie
-// that it does not have (x has 24 bits, (k + 1/2) d at most 16: they differ by more than half a unit of the quotient), so
-// rint of it is the nearest level of the exact quotient. NaN counts as 0 and infinities saturate the scale: whatever a row holds, the
-// cache stays finite, and no masked position can hurt another.
-__device__ __forceinline__ void quantize_lane(float x, __half* d, int* level) {
-    x = x == x ? x : 0.0f;
-    float hi = x, lo = x;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-    }
-    const float m = hi >= -lo ? hi : lo;
-    *d = __float2half_rn(fminf(fmaxf(m * -0.125f, -65504.0f), 65504.0f));
-    const float f = __half2float(*d);
-    *level = f == 0.0f ? 8 : 8 + (int)fminf(fmaxf(rintf(__fdiv_rn(x, f)), -8.0f), 7.0f);
-}
-
-// Rows of k and v into the cache: a warp takes one block of one row and head. Bound: latency, a few KB a row; a lane's nibble goes
-// through shuffles to the lane that owns its word.
-__global__ void kv4_append_kernel(Kv4 c, const float* __restrict__ k, const float* __restrict__ v, int ldkv, KvRows rows, const int* __restrict__ lens) {
+// Rows of k and v into the cache: a warp takes up to four blocks of one row and head, eight lanes a block. Bound: the bytes of long
+// prompts, latency of short ones.
+__global__ void __launch_bounds__(256) kv4_append_kernel(Kv4 c, const float* __restrict__ k, const float* __restrict__ v, int ldkv, KvRows rows, const int* __restrict__ lens) {
     const int lane = threadIdx.x & 31, seq = blockIdx.z, h = blockIdx.y, first = rows.start[seq], n = rows.start[seq + 1] - first;
     const int len = lens[seq];
     if (len < 0 || len > c.cap - n) return;
-    const int warps = gridDim.x * (blockDim.x >> 5);
-    for (int w = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); w < n * c.nb; w += warps) {
-        const int i = w / c.nb, b = w % c.nb, pos = len + i;
-        const size_t in = (size_t)(first + i) * ldkv + h * c.dim() + b * kKvBlock + lane, row = c.row(seq, h, pos);
+    const int warps = gridDim.x * (blockDim.x >> 5), parts = (c.nb + 3) / 4;
+    for (int w = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); w < n * parts; w += warps) {
+        const int i = w / parts, b = w % parts * 4 + (lane >> 3), pos = len + i, e = lane & 7;
+        const bool in = b < c.nb;
+        const size_t at = (size_t)(first + i) * ldkv + h * c.dim() + b * kKvBlock + 4 * e, row = c.row(seq, h, pos);
+        const float4 none = make_float4(0.0f, 0.0f, 0.0f, 0.0f), kx = in ? *(const float4*)(k + at) : none, vx = in ? *(const float4*)(v + at) : none;
         __half d;
-        int level;
-        quantize_lane(k[in], &d, &level);
-        // lane 8 t + i holds nibble i of word t
-        unsigned word = (unsigned)level << (4 * (lane & 7));
-#pragma unroll
-        for (int o = 4; o > 0; o >>= 1) word |= __shfl_xor_sync(0xffffffffu, word, o);
-        if ((lane & 7) == 0) c.kq[row * (c.nb * 4) + (lane >> 3) * c.nb + b] = word;
-        if (lane == 0) c.kd[row * c.nb + b] = d;
-        quantize_lane(v[in], &d, &level);
-        // lane 8 j + g holds nibble j of the half word of g
-        word = (unsigned)level << (4 * (lane >> 3));
-#pragma unroll
-        for (int o = 16; o > 4; o >>= 1) word |= __shfl_xor_sync(0xffffffffu, word, o);
-        if (lane < 8) {
-            const size_t pair = c.row(seq, h, pos & ~1) >> 1;
-            ((uint16_t*)c.vq)[2 * (pair * (c.nb * 8) + lane * c.nb + b) + (pos & 1)] = (uint16_t)word;
+        int level[4];
+        quantize4(kx, &d, level);
+        const uint32_t word = key_word(level, lane);
+        if (in && !(e & 1)) c.kq[row * (c.nb * 4) + (e >> 1) * c.nb + b] = word;
+        if (in && !e) c.kd[row * c.nb + b] = d;
+        quantize4(vx, &d, level);
+        const uint2 half = value_halves(level, lane);
+        if (in && e < 2) {
+            uint16_t* to = (uint16_t*)c.vq + 2 * ((row >> 1) * (c.nb * 8) + (4 * e) * c.nb + b) + (pos & 1);
+            to[0] = (uint16_t)half.x; to[2 * c.nb] = (uint16_t)(half.x >> 16);
+            to[4 * c.nb] = (uint16_t)half.y; to[6 * c.nb] = (uint16_t)(half.y >> 16);
         }
-        if (lane == 0) c.vd[row * c.nb + b] = d;
+        if (in && !e) c.vd[row * c.nb + b] = d;
     }
 }
 
@@ -153,7 +132,7 @@ __global__ void __launch_bounds__(ET) kv4_evict_kernel(Kv4 src, Kv4 dst, const i
 }  // namespace
 
 int launch_kv4_append(const Kv4& c, const float* k, const float* v, int ldkv, const KvRows& rows, int max_rows, const int* lens, cudaStream_t st) {
-    const long long warps = (long long)max_rows * c.nb;
+    const long long warps = (long long)max_rows * ((c.nb + 3) / 4);
     const dim3 grid((unsigned)std::min<long long>((warps + 7) / 8, 4096), c.n_kv, c.n_seq);
     kv4_append_kernel<<<grid, 256, 0, st>>>(c, k, v, ldkv, rows, lens);
     FC_LAUNCHED();

@@ -108,6 +108,8 @@ __global__ void __launch_bounds__(AT) kv4_mass_kernel(Kv4 c, Kv4Attend a, KvRows
 }  // namespace
 
 int launch_kv4_attend(const Kv4& c, const Kv4Attend& a, const KvRows& rows, int max_rows, int device, cudaStream_t st) {
+    const bool step = kv4_step_covers(c, a.group, max_rows);
+    if (step && (!a.mass || max_rows * a.group <= 8)) return launch_kv4_step(c, a, rows, max_rows, nullptr, device, st);
     if (a.k) FC_TRY(launch_kv4_append(c, a.k, a.v, a.ldkv, rows, max_rows, a.lens, st));
     CallScratch scratch;
     const int heads = c.n_kv * a.group;
