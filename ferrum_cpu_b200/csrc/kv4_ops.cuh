@@ -21,6 +21,9 @@ int launch_kv4_append(const Kv4& c, const float* k, const float* v, int ldkv, co
 // kv4_step.cu: few query rows a key / value head; stats: where a row's maximum (base 2) and sum go, if another kernel adds up its weights.
 bool kv4_step_covers(const Kv4& c, int group, int max_rows);
 int launch_kv4_step(const Kv4& c, const Kv4Attend& a, const KvRows& rows, int max_rows, float2* stats, int device, cudaStream_t st);
+// kv4_prompt.cu: any number of them; and the weights that the positions receive, from such statistics.
+int launch_kv4_prompt(const Kv4& c, const Kv4Attend& a, const KvRows& rows, int max_rows, float2* stats, int device, cudaStream_t st);
+int launch_kv4_weights(const Kv4& c, const Kv4Attend& a, const KvRows& rows, const float2* stats, cudaStream_t st);
 int launch_kv4_attend(const Kv4& c, const Kv4Attend& a, const KvRows& rows, int max_rows, int device, cudaStream_t st);
 
 }  // namespace fc
