@@ -38,24 +38,34 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(Kv4 c, const float* __r
     }
 }
 
-// Positions from[seq] .. + n of every sequence as the values that they stand for: out [n_seq][n][n_kv][dim], zeros outside the cache.
-__global__ void kv4_read_kernel(Kv4 c, const int* __restrict__ from, int n, float* __restrict__ k, float* __restrict__ v) {
-    const int dim = c.dim(), seq = blockIdx.y, base = from ? from[seq] : 0;
-    const size_t all = (size_t)n * c.n_kv * dim;
-    for (size_t e = (size_t)blockIdx.x * blockDim.x + threadIdx.x; e < all; e += (size_t)gridDim.x * blockDim.x) {
-        const int ch = (int)(e % dim), h = (int)(e / dim % c.n_kv), i = (int)(e / dim / c.n_kv);
+// Positions from[seq] .. + n of every sequence as the values that they stand for: out [n_seq][n][n_kv][dim], zeros outside the cache. A thread
+// writes eight channels of a row, of keys from one word, of values from the nibble j of eight half words. Bound: the bytes written.
+__global__ void __launch_bounds__(256) kv4_read_kernel(Kv4 c, const int* __restrict__ from, int n, float* __restrict__ k, float* __restrict__ v) {
+    const int parts = c.nb * 4, seq = blockIdx.y, base = from ? from[seq] : 0;
+    const size_t all = (size_t)n * c.n_kv * parts;
+    for (size_t e = (size_t)blockIdx.x * blockDim.x + threadIdx.x; e < 2 * all; e += (size_t)gridDim.x * blockDim.x) {
+        const bool values = e >= all;
+        const size_t at = values ? e - all : e;
+        const int part = (int)(at % parts), b = part >> 2, t = part & 3, h = (int)(at / parts % c.n_kv), i = (int)(at / parts / c.n_kv);
         const long long pos = (long long)base + i;
-        float kx = 0.0f, vx = 0.0f;
+        float x[8] = {};
         if (pos >= 0 && pos < c.cap) {
-            const int b = ch / 32, r = ch % 32;
-            const size_t row = c.row(seq, h, (int)pos), pair = c.row(seq, h, (int)pos & ~1) >> 1;
-            const unsigned kw = c.kq[row * (c.nb * 4) + (r >> 3) * c.nb + b];
-            const unsigned vw = ((const uint16_t*)c.vq)[2 * (pair * (c.nb * 8) + (r & 7) * c.nb + b) + (pos & 1)];
-            kx = __half2float(c.kd[row * c.nb + b]) * (float)((int)(kw >> (4 * (r & 7)) & 15) - 8);
-            vx = __half2float(c.vd[row * c.nb + b]) * (float)((int)(vw >> (4 * (r >> 3)) & 15) - 8);
+            const size_t row = c.row(seq, h, (int)pos);
+            if (values) {
+                const uint16_t* w = (const uint16_t*)c.vq + 2 * ((row >> 1) * (c.nb * 8) + b) + (pos & 1);
+                const float d = __half2float(c.vd[row * c.nb + b]);
+#pragma unroll
+                for (int g = 0; g < 8; ++g) x[g] = d * (float)((int)(w[2 * g * c.nb] >> (4 * t) & 15) - 8);
+            } else {
+                const uint32_t w = c.kq[row * (c.nb * 4) + t * c.nb + b];
+                const float d = __half2float(c.kd[row * c.nb + b]);
+#pragma unroll
+                for (int g = 0; g < 8; ++g) x[g] = d * (float)((int)(w >> (4 * g) & 15) - 8);
+            }
         }
-        k[(size_t)seq * all + e] = kx;
-        v[(size_t)seq * all + e] = vx;
+        float4* to = (float4*)((values ? v : k) + ((size_t)seq * all + at) * 8);
+        to[0] = make_float4(x[0], x[1], x[2], x[3]);
+        to[1] = make_float4(x[4], x[5], x[6], x[7]);
     }
 }
 
@@ -66,67 +76,148 @@ __device__ __forceinline__ unsigned weight_key(float w) {
     return w != w ? 0u : b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u);
 }
 
-constexpr int ET = 512;
+constexpr int ET = 512, BINS = 2048, KEYS = 16384, LISTED = 2048;
+struct EvictShared {
+    unsigned key[KEYS + KEYS / 32];
+    unsigned bins[BINS];
+    int src[LISTED];                               // where the rows of a window of dst come from
+    int warp_n[ET / 32], warp_t[ET / 32];
+    int digit, above;
+};
 
-// One CTA a (sequence, head): the key of the last position that is kept by bisection, then the kept positions in order.
-__global__ void __launch_bounds__(ET) kv4_evict_kernel(Kv4 src, Kv4 dst, const int* __restrict__ lens, int* __restrict__ lens_out, int budget, int recent,
-                                                       const float* __restrict__ mass, float* __restrict__ mass_out, int* __restrict__ kept) {
-    __shared__ int found[ET / 32], base_more, base_tie;
-    const int tid = threadIdx.x, h = blockIdx.x, seq = blockIdx.y, head = seq * src.n_kv + h;
+// What stays of a (sequence, head), shared by gridDim.x CTAs. Each finds the key of the last position that stays for itself (three passes
+// of 11, 11 and 10 bits over the keys, in shared memory where they fit): the row of weights is short next to what is moved, and no CTA has to
+// wait for another. Then each brings a range of dst's rows. Bound: latency, and the bytes moved of long caches.
+__global__ void __launch_bounds__(ET, 2) kv4_evict_kernel(Kv4 src, Kv4 dst, const int* __restrict__ lens, int* __restrict__ lens_out, int budget, int recent,
+                                                          const float* __restrict__ mass, float* __restrict__ mass_out, int* __restrict__ kept) {
+    extern __shared__ __align__(16) char raw[];
+    EvictShared& s = *(EvictShared*)raw;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, h = blockIdx.y, seq = blockIdx.z, head = seq * src.n_kv + h;
     int len = lens[seq];
     len = len < 0 ? 0 : min(len, src.cap);
     const int left = min(len, budget);
-    if (tid == 0 && h == 0) lens_out[seq] = left;
+    if (tid == 0 && h == 0 && blockIdx.x == 0) lens_out[seq] = left;
+    // this CTA's rows of dst, an even number from an even one on
+    const int share = ((left + (int)gridDim.x - 1) / (int)gridDim.x + 1) & ~1, d0 = min(left, (int)blockIdx.x * share), d1 = min(left, d0 + share);
+    for (int j = max(left, (int)blockIdx.x * ((budget + (int)gridDim.x - 1) / (int)gridDim.x)) + tid; kept && j < min(budget, ((int)blockIdx.x + 1) * ((budget + (int)gridDim.x - 1) / (int)gridDim.x)); j += ET)
+        kept[(size_t)head * budget + j] = -1;
+    if (d0 >= d1) return;
     const float* m = mass + (size_t)head * src.cap;
     const bool all = len <= budget;
-    const int old = all ? len : len - recent, want = all ? old : budget - recent;
-    auto count = [&](unsigned at) {
-        int n = 0;
-        for (int j = tid; j < old; j += ET) n += weight_key(m[j]) >= at;
-        for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
-        __syncthreads();
-        if ((tid & 31) == 0) found[tid >> 5] = n;
-        __syncthreads();
-        n = 0;
-        for (int w = 0; w < ET / 32; ++w) n += found[w];
-        return n;
-    };
+    const int old = all ? 0 : len - recent, want = budget - recent;      // of the first `old` positions the `want` heaviest
+    const bool fits = old <= KEYS;
+    auto slot = [](int j) { return j + (j >> 5); };
+    if (fits)
+        for (int j = tid; j < old; j += ET) s.key[slot(j)] = weight_key(m[j]);
+    auto key = [&](int j) { return fits ? s.key[slot(j)] : weight_key(__ldg(m + j)); };
     unsigned cut = 0;
-    for (int bit = 31; bit >= 0 && !all; --bit)
-        if (count(cut | (1u << bit)) >= want) cut |= 1u << bit;
-    const int more = all ? 0 : cut == 0xffffffffu ? 0 : count(cut + 1), ties = want - more;
-    if (tid == 0) base_more = base_tie = 0;
-    __syncthreads();
-    for (int j0 = 0; j0 < len; j0 += ET) {
-        const int j = j0 + tid;
-        const unsigned key = j < old ? weight_key(m[j]) : 0u;
-        const bool sure = j < len && (all || j >= old || (want > 0 && key > cut)), tie = !all && want > 0 && j < old && key == cut;
-        // how many of either kind come before j
-        const unsigned ms = __ballot_sync(0xffffffffu, sure), mt = __ballot_sync(0xffffffffu, tie), below = (1u << (tid & 31)) - 1;
-        __syncthreads();
-        if ((tid & 31) == 0) found[tid >> 5] = __popc(ms) | __popc(mt) << 16;
-        __syncthreads();
-        int s = base_more + __popc(ms & below), t = base_tie + __popc(mt & below), all_s = 0, all_t = 0;
-        for (int w = 0; w < ET / 32; ++w) {
-            if (w < (tid >> 5)) { s += found[w] & 0xffff; t += found[w] >> 16; }
-            all_s += found[w] & 0xffff; all_t += found[w] >> 16;
+    int ties = want;                               // how many of those at the cut stay, the first ones
+    if (!all && want > 0) {
+        int shift = 21, width = 11;
+        for (int pass = 0; pass < 3; ++pass) {
+            for (int b = tid; b < BINS; b += ET) s.bins[b] = 0;
+            __syncthreads();
+            const unsigned high = pass ? cut >> (shift + width) : 0;
+            for (int j = tid; j < old; j += ET) {
+                const unsigned k = key(j);
+                if (pass == 0 || k >> (shift + width) == high) atomicAdd(&s.bins[k >> shift & ((1u << width) - 1)], 1u);
+            }
+            __syncthreads();
+            // from the largest digit down: four a thread
+            int n[4], sum = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) { n[i] = (int)s.bins[BINS - 1 - (4 * tid + i)]; sum += n[i]; }
+            int incl = sum;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int x = __shfl_up_sync(0xffffffffu, incl, o);
+                if (lane >= o) incl += x;
+            }
+            if (lane == 31) s.warp_n[warp] = incl;
+            __syncthreads();
+            int before = incl - sum;
+            for (int w = 0; w < warp; ++w) before += s.warp_n[w];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (before < ties && before + n[i] >= ties) { s.digit = BINS - 1 - (4 * tid + i); s.above = before; }
+                before += n[i];
+            }
+            __syncthreads();
+            cut |= (unsigned)s.digit << shift;
+            ties -= s.above;
+            width = pass == 1 ? 10 : 11;
+            shift -= width;
+            if (shift < 0) shift = 0;
         }
-        if (sure || (tie && t < ties)) {
-            const int to = s + min(t, ties);
-            const size_t a = src.row(seq, h, j), b = dst.row(seq, h, to);
-            for (int w = 0; w < src.nb * 4; ++w) dst.kq[b * (src.nb * 4) + w] = src.kq[a * (src.nb * 4) + w];
-            const uint16_t* va = (const uint16_t*)src.vq + (a >> 1) * (src.nb * 16) + (a & 1);
-            uint16_t* vb = (uint16_t*)dst.vq + (b >> 1) * (src.nb * 16) + (b & 1);
-            for (int w = 0; w < src.nb * 8; ++w) vb[2 * w] = va[2 * w];
-            for (int w = 0; w < src.nb; ++w) { dst.kd[b * src.nb + w] = src.kd[a * src.nb + w]; dst.vd[b * src.nb + w] = src.vd[a * src.nb + w]; }
-            if (mass_out) mass_out[(size_t)head * dst.cap + to] = m[j];
-            if (kept) kept[(size_t)head * budget + to] = j;
-        }
-        __syncthreads();
-        if (tid == 0) { base_more += all_s; base_tie += all_t; }
-        __syncthreads();
     }
-    for (int j = left + tid; kept && j < budget; j += ET) kept[(size_t)head * budget + j] = -1;
+    __syncthreads();
+    // thread t walks positions [t * per, ..): how many of them are sure to stay, and how many are at the cut
+    const int per = (old + ET - 1) / ET, j0 = min(old, tid * per), j1 = min(old, j0 + per);
+    int sure = 0, tie = 0;
+    if (want > 0)
+        for (int j = j0; j < j1; ++j) {
+            const unsigned k = key(j);
+            sure += k > cut;
+            tie += k == cut;
+        }
+    int is = sure, it = tie;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int a = __shfl_up_sync(0xffffffffu, is, o), b = __shfl_up_sync(0xffffffffu, it, o);
+        if (lane >= o) { is += a; it += b; }
+    }
+    if (lane == 31) { s.warp_n[warp] = is; s.warp_t[warp] = it; }
+    __syncthreads();
+    int s0 = is - sure, t0 = it - tie;
+    for (int w = 0; w < warp; ++w) { s0 += s.warp_n[w]; t0 += s.warp_t[w]; }
+    const int first = s0 + min(t0, ties), last = s0 + sure + min(t0 + tie, ties);    // this thread's rows of dst
+    const size_t da = dst.row(seq, h, 0), sa = src.row(seq, h, 0);
+    const int nb = src.nb;
+    for (int w0 = d0; w0 < d1; w0 += LISTED) {
+        const int w1 = min(d1, w0 + LISTED), rows = w1 - w0;
+        __syncthreads();
+        if (!all && want > 0 && first < w1 && last > w0) {
+            int to = first, t = t0;
+            for (int j = j0; j < j1; ++j) {
+                const unsigned k = key(j);
+                if (k > cut || (k == cut && t++ < ties)) {
+                    if (to >= w0 && to < w1) s.src[to - w0] = j;
+                    ++to;
+                }
+            }
+        }
+        // the recent ones, or all
+        const int body = all ? 0 : want;
+        for (int to = max(w0, body) + tid; to < w1; to += ET) s.src[to - w0] = all ? to : to - body + old;
+        __syncthreads();
+        for (int e = tid; e < rows * nb; e += ET) {
+            const int i = e / nb, q = e % nb;
+            ((uint4*)(dst.kq + (da + w0 + i) * (nb * 4)))[q] = __ldg((const uint4*)(src.kq + (sa + s.src[i]) * (nb * 4)) + q);
+        }
+        const int pairs = rows >> 1;
+        for (int e = tid; e < pairs * 2 * nb; e += ET) {
+            const int i = e / (2 * nb), q = e % (2 * nb), a = s.src[2 * i], b = s.src[2 * i + 1];
+            const uint4 x = __ldg((const uint4*)(src.vq + ((sa + a) >> 1) * (nb * 8)) + q), y = __ldg((const uint4*)(src.vq + ((sa + b) >> 1) * (nb * 8)) + q);
+            const unsigned pick = (a & 1 ? 0x32 : 0x10) | (b & 1 ? 0x7600 : 0x5400);
+            ((uint4*)(dst.vq + ((da + w0) / 2 + i) * (nb * 8)))[q] =
+                make_uint4(__byte_perm(x.x, y.x, pick), __byte_perm(x.y, y.y, pick), __byte_perm(x.z, y.z, pick), __byte_perm(x.w, y.w, pick));
+        }
+        if (rows & 1) {                            // a last row alone: what lies behind it stays as it was
+            const int a = s.src[rows - 1];
+            const uint16_t* x = (const uint16_t*)(src.vq + ((sa + a) >> 1) * (nb * 8)) + (a & 1);
+            uint16_t* y = (uint16_t*)(dst.vq + ((da + w1 - 1) / 2) * (nb * 8));
+            for (int e = tid; e < 8 * nb; e += ET) y[2 * e] = x[2 * e];
+        }
+        for (int e = tid; e < rows * nb; e += ET) {
+            const int i = e / nb, q = e % nb;
+            dst.kd[(da + w0) * nb + e] = src.kd[(sa + s.src[i]) * nb + q];
+            dst.vd[(da + w0) * nb + e] = src.vd[(sa + s.src[i]) * nb + q];
+        }
+        for (int i = tid; i < rows; i += ET) {
+            if (mass_out) mass_out[(size_t)head * dst.cap + w0 + i] = m[s.src[i]];
+            if (kept) kept[(size_t)head * budget + w0 + i] = s.src[i];
+        }
+    }
 }
 
 }  // namespace
@@ -249,7 +340,8 @@ int fc_kv4_read_dev(const fc_kv4* c, const int32_t* from, int n, float* k, float
     if (n < 0) return fail(FC_E_SHAPE, "fc_kv4_read_dev: n = %d", n);
     if (!n) return FC_OK;
     FC_TRY(make_device(c->device));
-    const size_t all = (size_t)n * c->c.n_kv * c->c.dim();
+    if (!aligned16(k) || !aligned16(v)) return fail(FC_E_ARG, "fc_kv4_read_dev: k and v must be 16-byte aligned");
+    const size_t all = (size_t)n * c->c.n_kv * c->c.nb * 8;
     const dim3 grid((unsigned)std::min<size_t>((all + 255) / 256, 148 * 16), c->c.n_seq);
     kv4_read_kernel<<<grid, 256, 0, (cudaStream_t)stream>>>(c->c, from, n, k, v);
     FC_LAUNCHED();
@@ -266,7 +358,16 @@ int fc_kv4_evict_dev(const fc_kv4* src, fc_kv4* dst, const int32_t* lens, int32_
     if (budget <= 0 || recent < 0 || recent > budget) return fail(FC_E_SHAPE, "fc_kv4_evict_dev: budget %d, recent %d", budget, recent);
     if (budget > b.cap) return fail(FC_E_DIM, "fc_kv4_evict_dev: a budget of %d does not fit %d positions", budget, b.cap);
     FC_TRY(make_device(src->device));
-    kv4_evict_kernel<<<dim3(a.n_kv, a.n_seq), ET, 0, (cudaStream_t)stream>>>(a, b, lens, lens_out, budget, recent, mass, mass_out, kept);
+    static bool attr_set[64] = {};
+    if (src->device >= 64 || !attr_set[src->device]) {
+        FC_CUDA(cudaFuncSetAttribute(kv4_evict_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(EvictShared)));
+        if (src->device < 64) attr_set[src->device] = true;
+    }
+    // CTAs that share a head: as many as are resident, 64 rows of dst each at least
+    const long long heads = (long long)a.n_kv * a.n_seq;
+    int share = 1;
+    while (share < 32 && heads * share * 2 <= 296 && budget >= share * 2 * 64) share *= 2;
+    kv4_evict_kernel<<<dim3(share, a.n_kv, a.n_seq), ET, sizeof(EvictShared), (cudaStream_t)stream>>>(a, b, lens, lens_out, budget, recent, mass, mass_out, kept);
     FC_LAUNCHED();
     return FC_OK;
 }

@@ -553,7 +553,7 @@ typedef struct {
     int32_t top_k;
     float top_p, min_p;
 } fc_row_sampling;
-/* One draw from each of n_rows rows of `vocab` logits (2^24 at most), ld floats apart, with given random numbers u [n_rows] in [0, 1).
+/* One draw from each of n_rows rows of `vocab` logits (2^20 at most), ld floats apart, with given random numbers u [n_rows] in [0, 1).
  * w = exp((l - max) / temperature) in 64 bits. As in fc_sample_logits, all of a tie at a cut stays: ids that are not below the top_k-th
  * largest logit, nor below the largest logit down to which the mass reaches top_p of the whole row; and w >= min_p. Of what
  * stays, weights under 2^-40 are nothing. The token is the first id, in index order, at which the running mass reaches u
