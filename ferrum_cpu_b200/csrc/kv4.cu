@@ -78,7 +78,7 @@ __device__ __forceinline__ unsigned weight_key(float w) {
 
 constexpr int ET = 512, BINS = 2048, KEYS = 16384, LISTED = 2048;
 struct EvictShared {
-    unsigned key[KEYS + KEYS / 32];
+    unsigned key[KEYS];
     unsigned bins[BINS];
     int src[LISTED];                               // where the rows of a window of dst come from
     int warp_n[ET / 32], warp_t[ET / 32];
@@ -106,10 +106,9 @@ __global__ void __launch_bounds__(ET, 2) kv4_evict_kernel(Kv4 src, Kv4 dst, cons
     const bool all = len <= budget;
     const int old = all ? 0 : len - recent, want = budget - recent;      // of the first `old` positions the `want` heaviest
     const bool fits = old <= KEYS;
-    auto slot = [](int j) { return j + (j >> 5); };
     if (fits)
-        for (int j = tid; j < old; j += ET) s.key[slot(j)] = weight_key(m[j]);
-    auto key = [&](int j) { return fits ? s.key[slot(j)] : weight_key(__ldg(m + j)); };
+        for (int j = tid; j < old; j += ET) s.key[j] = weight_key(m[j]);
+    auto key = [&](int j) { return fits ? s.key[j] : weight_key(__ldg(m + j)); };
     unsigned cut = 0;
     int ties = want;                               // how many of those at the cut stay, the first ones
     if (!all && want > 0) {
@@ -151,8 +150,8 @@ __global__ void __launch_bounds__(ET, 2) kv4_evict_kernel(Kv4 src, Kv4 dst, cons
         }
     }
     __syncthreads();
-    // thread t walks positions [t * per, ..): how many of them are sure to stay, and how many are at the cut
-    const int per = (old + ET - 1) / ET, j0 = min(old, tid * per), j1 = min(old, j0 + per);
+    // thread t walks positions [t * per, ..) (an odd stride meets every bank): how many of them are sure to stay, and how many are at the cut
+    const int per = ((old + ET - 1) / ET) | 1, j0 = min(old, tid * per), j1 = min(old, j0 + per);
     int sure = 0, tie = 0;
     if (want > 0)
         for (int j = j0; j < j1; ++j) {

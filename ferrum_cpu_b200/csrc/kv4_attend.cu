@@ -19,7 +19,7 @@ int launch_kv4_attend(const Kv4& c, const Kv4Attend& a, const KvRows& rows, int 
         if (a.k) FC_TRY(launch_kv4_append(c, a.k, a.v, a.ldkv, rows, max_rows, a.lens, st));
         FC_TRY(launch_kv4_prompt(c, a, rows, max_rows, stats, device, st));
     }
-    return a.mass ? launch_kv4_weights(c, a, rows, stats, st) : FC_OK;
+    return a.mass ? launch_kv4_weights(c, a, rows, max_rows, stats, device, st) : FC_OK;
 }
 
 }  // namespace fc

@@ -45,6 +45,10 @@ __device__ __forceinline__ void planes_of(float x, float y, uint32_t* hi, uint32
     *hi = *(const uint32_t*)&h;
     *lo = *(const uint32_t*)&l;
 }
+// Weights are kept times 2^6 and the scales they meet are brought to [2^7, 2^8): the product stays below 2^14, and what f16 cannot hold is
+// 2^-31 of the largest weight and 2^-32 of the largest scale.
+constexpr float kLift = 6.0f;
+constexpr int kScaleLift = 7;
 // 2^e, -126 <= e <= 127
 __device__ __forceinline__ float exp2i(int e) { return __int_as_float((e + 127) << 23); }
 // The power of two that brings values of at most `top` (finite, >= 0) into [2^13, 2^14); 2^126 at most.

@@ -23,7 +23,7 @@ bool kv4_step_covers(const Kv4& c, int group, int max_rows);
 int launch_kv4_step(const Kv4& c, const Kv4Attend& a, const KvRows& rows, int max_rows, float2* stats, int device, cudaStream_t st);
 // kv4_prompt.cu: any number of them; and the weights that the positions receive, from such statistics.
 int launch_kv4_prompt(const Kv4& c, const Kv4Attend& a, const KvRows& rows, int max_rows, float2* stats, int device, cudaStream_t st);
-int launch_kv4_weights(const Kv4& c, const Kv4Attend& a, const KvRows& rows, const float2* stats, cudaStream_t st);
+int launch_kv4_weights(const Kv4& c, const Kv4Attend& a, const KvRows& rows, int max_rows, const float2* stats, int device, cudaStream_t st);
 int launch_kv4_attend(const Kv4& c, const Kv4Attend& a, const KvRows& rows, int max_rows, int device, cudaStream_t st);
 
 }  // namespace fc

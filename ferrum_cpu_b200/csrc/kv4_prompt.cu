@@ -5,7 +5,7 @@
 // warps. S = q K^T: exact levels against two f16 planes of q, a block's sum times its scale in f32. O = P V: exact levels against two
 // planes of the weight times the value's scale. That product is formed in f16 pairs: with p = ph + pl, the high plane is
 // rn(ph d) and the low one (ph d - rn(ph d), exact in a fused multiply-add) + pl d. So that it stays within f16, a position's scales are
-// divided by the power of two 2^e of the largest of its blocks, and e is added to its score: the running maximum is that of s + e, and
+// divided by the power of two 2^e of the largest of its blocks (and times 2^kScaleLift), and e is added to its score: the running maximum is that of s + e, and
 // the sum takes 2^-e back. Sums of products start from zero in every tile and are added to the row's in f32, because
 // the tensor core truncates.
 //
@@ -22,7 +22,6 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int KT = 64;                           // positions a tile
-constexpr float kLift = 13.0f;                   // weights are at most 2^13
 
 template <int NB>
 struct PromptShape {
@@ -50,31 +49,46 @@ __device__ __forceinline__ uint32_t hmadd2u(uint32_t a, uint32_t b, uint32_t c) 
     return *(const uint32_t*)&r;
 }
 
-// Two rows of q as fragments (rows g and g + 8 of 16): channels 32 b + 8 t .. + 7, brought to [2^13, 2^14) by a power of two each, whose
-// inverses come back in inv.
+// Channels 32 b + 8 t .. + 7 of two rows of q (rows g and g + 8 of 16), as they are; zeros for a row that is none.
 template <int NB>
-__device__ __forceinline__ void query_planes(const float* q0, const float* q1, float scale, uint32_t (&qh)[NB][8], uint32_t (&ql)[NB][8], float (&inv)[2]) {
+__device__ __forceinline__ void query_ask(const float* q0, const float* q1, float4 (&x)[2][NB][2]) {
+    const float4 zero = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
         const float* q = r ? q1 : q0;
-        float x[NB][8], top = 0.0f;
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            const float4 zero = make_float4(0.0f, 0.0f, 0.0f, 0.0f), lo = q ? *(const float4*)(q + 32 * b) : zero, hi = q ? *(const float4*)(q + 32 * b + 4) : zero;
-            const float v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+        for (int b = 0; b < NB; ++b)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) { x[b][j] = v[j] * scale; top = fmaxf(top, fabsf(x[b][j])); }
-        }
+            for (int u = 0; u < 2; ++u) x[r][b][u] = q ? *(const float4*)(q + 32 * b + 4 * u) : zero;
+    }
+}
+// As fragments of two planes, brought to [2^13, 2^14) by a power of two a row, whose inverses come back in inv. Registers 4 u + {0: row g,
+// 1: row g + 8} of a block hold the nibbles 2 u, {2, 3} the nibbles 2 u + 1.
+template <int NB>
+__device__ __forceinline__ void query_planes(const float4 (&x)[2][NB][2], float scale, uint32_t (&qh)[NB][8], uint32_t (&ql)[NB][8], float (&inv)[2]) {
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+        float top = 0.0f;
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const float4 v = x[r][b][u];
+                top = fmaxf(fmaxf(top, fmaxf(fabsf(v.x * scale), fabsf(v.y * scale))), fmaxf(fabsf(v.z * scale), fabsf(v.w * scale)));
+            }
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
         const int shift = plane_shift(top);
         const float up = exp2i(shift);
         inv[r] = exp2i(-shift);
-        // fragment u of a block: registers 4 u + {0: row g, 1: row g + 8} of nibbles 2 u, {2, 3} of nibbles 2 u + 1
 #pragma unroll
-        for (int b = 0; b < NB; ++b)
+        for (int b = 0; b < NB; ++b) {
+            const float4 lo = x[r][b][0], hi = x[r][b][1];
+            const float v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
-            for (int j = 0; j < 4; ++j) planes_of(x[b][j] * up, x[b][j + 4] * up, &qh[b][4 * (j >> 1) + 2 * (j & 1) + r], &ql[b][4 * (j >> 1) + 2 * (j & 1) + r]);
+            for (int j = 0; j < 4; ++j)
+                planes_of(v[j] * scale * up, v[j + 4] * scale * up, &qh[b][4 * (j >> 1) + 2 * (j & 1) + r], &ql[b][4 * (j >> 1) + 2 * (j & 1) + r]);
+        }
     }
 }
 
@@ -136,7 +150,7 @@ __device__ __forceinline__ void tile_lay(char* buf, int tid, const RawTile<NB, P
         const int e = top > 0.0f ? (__float_as_int(top) >> 23) - 127 : 0;    // an f16 above 0 is a normal f32
         const float back = exp2i(-e);
 #pragma unroll
-        for (int b = 0; b < NB; ++b) ((__half*)(buf + S::VD))[b * KT + j] = __float2half_rn(d[b] * back);
+        for (int b = 0; b < NB; ++b) ((__half*)(buf + S::VD))[b * KT + j] = __float2half_rn(d[b] * back * (float)(1 << kScaleLift));
         ((float2*)(buf + S::EX))[j] = make_float2((float)e, back);
     }
 }
@@ -178,7 +192,9 @@ kv4_prompt_kernel(Kv4 c, Kv4Attend a, KvRows rows, int cs, float2* __restrict__ 
             const int i = (col0 + col) / a.group, head = h * a.group + (col0 + col) - i * a.group;
             return col < cols ? a.q + (size_t)(first + i) * a.ldq + (size_t)head * DIM + 8 * t : nullptr;
         };
-        query_planes<NB>(from(ca), from(cb), a.scale * 1.44269504f, qh, ql, inv);
+        float4 x[2][NB][2];
+        query_ask<NB>(from(ca), from(cb), x);
+        query_planes<NB>(x, a.scale * 1.44269504f, qh, ql, inv);
     }
     uint4* const qs = (uint4*)smem + warp * (NB * 4 * 32) + lane;     // [block][plane, fragment][lane]
     if (S::QS) {
@@ -333,7 +349,7 @@ kv4_prompt_kernel(Kv4 c, Kv4Attend a, KvRows rows, int cs, float2* __restrict__ 
         return stats[((size_t)first + i) * (c.n_kv * a.group) + h * a.group + (col0 + col) - i * a.group];
     };
     if (cs == 1) {
-        const float fa = la == 0.0f ? 0.0f : 1.0f / la, fb = lb == 0.0f ? 0.0f : 1.0f / lb;
+        const float one = 1.0f / (float)(1 << kScaleLift), fa = la == 0.0f ? 0.0f : one / la, fb = lb == 0.0f ? 0.0f : one / lb;
         if (ca < cols) {
             float* to = out + place(ca) + 2 * t;
 #pragma unroll
@@ -377,7 +393,7 @@ kv4_prompt_kernel(Kv4 c, Kv4Attend a, KvRows rows, int cs, float2* __restrict__ 
             l = fmaf(y.y, f, l);
             x.x = fmaf(v.x, f, x.x); x.y = fmaf(v.y, f, x.y); x.z = fmaf(v.z, f, x.z); x.w = fmaf(v.w, f, x.w);
         }
-        const float f = l == 0.0f ? 0.0f : 1.0f / l;
+        const float f = l == 0.0f ? 0.0f : 1.0f / (float)(1 << kScaleLift) / l;
         *(float4*)(out + place(col) + ch) = make_float4(x.x * f, x.y * f, x.z * f, x.w * f);
         if (ch == 0 && stats) stat(col) = make_float2(m == -INFINITY ? 0.0f : m - kLift, l);
     }
@@ -385,24 +401,24 @@ kv4_prompt_kernel(Kv4 c, Kv4Attend a, KvRows rows, int cs, float2* __restrict__ 
 }
 
 // ---- the weights that positions receive --------------------------------------------------------------------------
-constexpr int WW = 4, WCOLS = 32;                // warps; columns a pass
+constexpr int WW = 4, WCOLS = 16 * WW;           // warps; columns a pass
 template <int NB>
 struct WeightsShape {
     static constexpr int TILES = NB <= 4 ? 4 : 2, POS = 8 * TILES * WW;       // tiles of 8 positions a warp, positions a CTA
-    static constexpr int BUFS = NB <= 4 ? 2 : 1;
+    static constexpr int BUFS = NB <= 4 ? 2 : 1, BUF = WW * NB * 4 * 512 + WCOLS * 16, SMEM = BUFS * BUF;
 };
 
 template <int NB>
-__global__ void __launch_bounds__(32 * WW) kv4_weights_kernel(Kv4 c, Kv4Attend a, KvRows rows, const float2* __restrict__ stats) {
-    constexpr int DIM = NB * kKvBlock, TILES = WeightsShape<NB>::TILES, BUFS = WeightsShape<NB>::BUFS;
-    __shared__ uint4 qf[BUFS][2][NB * 4][32];       // [buffer][16 columns][block, plane and fragment][lane]
-    __shared__ float4 col_of[BUFS][WCOLS];          // 1 / power of two of q, maximum, 1 / sum, positions seen
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3, h = blockIdx.y, seq = blockIdx.z;
+__global__ void __launch_bounds__(32 * WW) kv4_weights_kernel(Kv4 c, Kv4Attend a, KvRows rows, int cs, const float2* __restrict__ stats) {
+    using S = WeightsShape<NB>;
+    constexpr int DIM = NB * kKvBlock, TILES = S::TILES, BUFS = S::BUFS;
+    extern __shared__ __align__(16) char smem[]; // [buffer]: fragments [16 columns][block, plane and fragment][lane], columns
+    __shared__ float part[S::POS];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3, rank = blockIdx.x % cs, h = blockIdx.y, seq = blockIdx.z;
     const int first = rows.start[seq], n = rows.start[seq + 1] - first, all_cols = n * a.group;
     const int len = a.lens[seq], end = a.k ? len + n : len;
-    if (n == 0 || len < 0 || len > c.cap - (a.k ? n : 0)) return;
-    const int j00 = blockIdx.x * (8 * TILES * WW), j0 = j00 + warp * (8 * TILES), base = end - n + 1;
-    if (j00 >= end) return;
+    const int j00 = blockIdx.x / cs * S::POS, j0 = j00 + warp * (8 * TILES), base = end - n + 1;
+    if (n == 0 || len < 0 || len > c.cap - (a.k ? n : 0) || j00 >= end) return;      // the whole cluster
     // levels and scales of the warp's positions
     uint32_t kf[TILES][NB][4];
     float2 kd[TILES][NB];
@@ -418,26 +434,33 @@ __global__ void __launch_bounds__(32 * WW) kv4_weights_kernel(Kv4 c, Kv4Attend a
         }
     }
     float sum[TILES][2] = {};
-    // the first column that sees any of the CTA's positions
+    // the first column that sees any of the CTA's positions; the ranks take turns
     const int col_first = max(0, j00 + 1 - base) * a.group / WCOLS * WCOLS;
+    auto from = [&](int col) {
+        const int i = col / a.group, head = h * a.group + col - i * a.group;
+        return col < all_cols ? a.q + (size_t)(first + i) * a.ldq + (size_t)head * DIM + 8 * t : nullptr;
+    };
+    float4 raw[2][NB][2];
+    int c0 = col_first + rank * WCOLS;
+    if (BUFS == 2 && c0 < all_cols) query_ask<NB>(from(c0 + warp * 16 + g), from(c0 + warp * 16 + g + 8), raw);
     int flip = 0;
-    for (int c0 = col_first; c0 < all_cols; c0 += WCOLS) {
-        // warps 0 and 1 lay 16 columns each
-        if (warp < 2) {
+    for (; c0 < all_cols; c0 += cs * WCOLS) {
+        char* const buf = smem + flip * S::BUF;
+        uint4* const qf = (uint4*)buf;
+        float4* const col_of = (float4*)(buf + WW * NB * 4 * 512);     // 1 / power of two of q, maximum, 1 / sum, positions seen
+        {
+            // every warp lays 16 columns
+            const int ca = c0 + warp * 16 + g;
             uint32_t qh[NB][8], ql[NB][8];
             float inv[2];
-            auto from = [&](int col) {
-                const int i = col / a.group, head = h * a.group + col - i * a.group;
-                return col < all_cols ? a.q + (size_t)(first + i) * a.ldq + (size_t)head * DIM + 8 * t : nullptr;
-            };
-            const int ca = c0 + warp * 16 + g;
-            query_planes<NB>(from(ca), from(ca + 8), a.scale * 1.44269504f, qh, ql, inv);
+            if (BUFS == 1) query_ask<NB>(from(ca), from(ca + 8), raw);
+            query_planes<NB>(raw, a.scale * 1.44269504f, qh, ql, inv);
 #pragma unroll
             for (int b = 0; b < NB; ++b)
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
-                    qf[flip][warp][b * 4 + u][lane] = make_uint4(qh[b][4 * u], qh[b][4 * u + 1], qh[b][4 * u + 2], qh[b][4 * u + 3]);
-                    qf[flip][warp][b * 4 + 2 + u][lane] = make_uint4(ql[b][4 * u], ql[b][4 * u + 1], ql[b][4 * u + 2], ql[b][4 * u + 3]);
+                    qf[(warp * (NB * 4) + b * 4 + u) * 32 + lane] = make_uint4(qh[b][4 * u], qh[b][4 * u + 1], qh[b][4 * u + 2], qh[b][4 * u + 3]);
+                    qf[(warp * (NB * 4) + b * 4 + 2 + u) * 32 + lane] = make_uint4(ql[b][4 * u], ql[b][4 * u + 1], ql[b][4 * u + 2], ql[b][4 * u + 3]);
                 }
             if (t == 0)
 #pragma unroll
@@ -445,34 +468,44 @@ __global__ void __launch_bounds__(32 * WW) kv4_weights_kernel(Kv4 c, Kv4Attend a
                     const int col = ca + 8 * r, i = col / a.group;
                     float2 st = make_float2(0.0f, 0.0f);
                     if (col < all_cols) st = stats[((size_t)first + i) * (c.n_kv * a.group) + h * a.group + col - i * a.group];
-                    col_of[flip][warp * 16 + 8 * r + g] = make_float4(inv[r], st.x, st.y == 0.0f ? 0.0f : 1.0f / st.y, __int_as_float(col < all_cols ? base + i : 0));
+                    col_of[warp * 16 + 8 * r + g] = make_float4(inv[r], st.x, st.y == 0.0f ? 0.0f : 1.0f / st.y, __int_as_float(col < all_cols ? base + i : 0));
                 }
+            const int next = ca + cs * WCOLS;
+            if (BUFS == 2 && c0 + cs * WCOLS < all_cols) query_ask<NB>(from(next), from(next + 8), raw);
         }
         __syncthreads();                         // with two buffers, the next pass's columns are laid while this one's are read
-#pragma unroll
-        for (int q = 0; q < 2; ++q) {
-            const float4 xa = col_of[flip][q * 16 + g], xb = col_of[flip][q * 16 + g + 8];
+#pragma unroll 1
+        for (int q = 0; q < WW; ++q) {
+            const float4 xa = col_of[q * 16 + g], xb = col_of[q * 16 + g + 8];
             const int seen_a = __float_as_int(xa.w), seen_b = __float_as_int(xb.w);
+            float s[TILES][4];
 #pragma unroll
-            for (int i = 0; i < TILES; ++i) {
-                float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            for (int i = 0; i < TILES; ++i)
 #pragma unroll
-                for (int b = 0; b < NB; ++b) {
-                    const uint4 x0 = qf[flip][q][b * 4][lane], x1 = qf[flip][q][b * 4 + 1][lane], y0 = qf[flip][q][b * 4 + 2][lane], y1 = qf[flip][q][b * 4 + 3][lane];
-                    const uint32_t h0[4] = {x0.x, x0.y, x0.z, x0.w}, h1[4] = {x1.x, x1.y, x1.z, x1.w}, r0[4] = {y0.x, y0.y, y0.z, y0.w}, r1[4] = {y1.x, y1.y, y1.z, y1.w};
+                for (int e = 0; e < 4; ++e) s[i][e] = 0.0f;
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                const uint4* f = qf + (q * (NB * 4) + b * 4) * 32 + lane;
+                const uint4 x0 = f[0], x1 = f[32], y0 = f[64], y1 = f[96];
+                const uint32_t h0[4] = {x0.x, x0.y, x0.z, x0.w}, h1[4] = {x1.x, x1.y, x1.z, x1.w}, r0[4] = {y0.x, y0.y, y0.z, y0.w}, r1[4] = {y1.x, y1.y, y1.z, y1.w};
+#pragma unroll
+                for (int i = 0; i < TILES; ++i) {
                     float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
                     mma16816(x, r0, kf[i][b][0], kf[i][b][1]);
                     mma16816(x, r1, kf[i][b][2], kf[i][b][3]);
                     mma16816(x, h0, kf[i][b][0], kf[i][b][1]);
                     mma16816(x, h1, kf[i][b][2], kf[i][b][3]);
-                    s[0] = fmaf(x[0], kd[i][b].x, s[0]);
-                    s[1] = fmaf(x[1], kd[i][b].y, s[1]);
-                    s[2] = fmaf(x[2], kd[i][b].x, s[2]);
-                    s[3] = fmaf(x[3], kd[i][b].y, s[3]);
+                    s[i][0] = fmaf(x[0], kd[i][b].x, s[i][0]);
+                    s[i][1] = fmaf(x[1], kd[i][b].y, s[i][1]);
+                    s[i][2] = fmaf(x[2], kd[i][b].x, s[i][2]);
+                    s[i][3] = fmaf(x[3], kd[i][b].y, s[i][3]);
                 }
+            }
+#pragma unroll
+            for (int i = 0; i < TILES; ++i) {
                 const int j = j0 + 8 * i + 2 * t;
-                sum[i][0] += (j < seen_a ? ex2(fmaf(s[0], xa.x, -xa.y)) * xa.z : 0.0f) + (j < seen_b ? ex2(fmaf(s[2], xb.x, -xb.y)) * xb.z : 0.0f);
-                sum[i][1] += (j + 1 < seen_a ? ex2(fmaf(s[1], xa.x, -xa.y)) * xa.z : 0.0f) + (j + 1 < seen_b ? ex2(fmaf(s[3], xb.x, -xb.y)) * xb.z : 0.0f);
+                sum[i][0] += (j < seen_a ? ex2(fmaf(s[i][0], xa.x, -xa.y)) * xa.z : 0.0f) + (j < seen_b ? ex2(fmaf(s[i][2], xb.x, -xb.y)) * xb.z : 0.0f);
+                sum[i][1] += (j + 1 < seen_a ? ex2(fmaf(s[i][1], xa.x, -xa.y)) * xa.z : 0.0f) + (j + 1 < seen_b ? ex2(fmaf(s[i][3], xb.x, -xb.y)) * xb.z : 0.0f);
             }
         }
         if (BUFS == 2) flip ^= 1;
@@ -487,9 +520,19 @@ __global__ void __launch_bounds__(32 * WW) kv4_weights_kernel(Kv4 c, Kv4Attend a
             float x = sum[i][r];
 #pragma unroll
             for (int w = 4; w < 32; w <<= 1) x += __shfl_xor_sync(0xffffffffu, x, w);
-            const int j = j0 + 8 * i + 2 * t + r;
-            if (g == 0 && j < end) mass[j] = (j < old ? mass[j] : 0.0f) + x;
+            if (g == 0) part[warp * (8 * TILES) + 8 * i + 2 * t + r] = x;
         }
+    // the ranks' sums, in their order
+    cg::cluster_group cluster = cg::this_cluster();
+    if (cs > 1) cluster.sync();
+    else __syncthreads();
+    const int j = j00 + tid;
+    if (rank == 0 && tid < S::POS && j < end) {
+        float x = 0.0f;
+        for (int r = 0; r < cs; ++r) x += cluster.map_shared_rank(part, r)[tid];
+        mass[j] = (j < old ? mass[j] : 0.0f) + x;
+    }
+    if (cs > 1) cluster.sync();                  // no rank leaves while another reads its memory
 }
 
 template <int NB>
@@ -520,8 +563,29 @@ int launch_prompt_t(const Kv4& c, const Kv4Attend& a, const KvRows& rows, int ma
     return FC_OK;
 }
 template <int NB>
-int launch_weights_t(const Kv4& c, const Kv4Attend& a, const KvRows& rows, const float2* stats, cudaStream_t st) {
-    kv4_weights_kernel<NB><<<dim3((c.cap + WeightsShape<NB>::POS - 1) / WeightsShape<NB>::POS, c.n_kv, c.n_seq), 32 * WW, 0, st>>>(c, a, rows, stats);
+int launch_weights_t(const Kv4& c, const Kv4Attend& a, const KvRows& rows, int max_rows, const float2* stats, int device, cudaStream_t st) {
+    using S = WeightsShape<NB>;
+    static bool attr_set[64] = {};
+    if (device >= 64 || !attr_set[device]) {
+        FC_CUDA(cudaFuncSetAttribute(kv4_weights_kernel<NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM));
+        if (device < 64) attr_set[device] = true;
+    }
+    const long long tiles = (c.cap + S::POS - 1) / S::POS, ctas = tiles * c.n_kv * c.n_seq, passes = ((long long)max_rows * a.group + WCOLS - 1) / WCOLS;
+    // the first positions are seen by all columns, the last by few: a cluster shares the columns, several rounds of CTAs even out the rest
+    int cs = 1;
+    while (cs < 8 && cs * 4 <= passes && ctas * cs < 148 * 8) cs *= 2;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(tiles * cs), c.n_kv, c.n_seq);
+    cfg.blockDim = dim3(32 * WW);
+    cfg.dynamicSmemBytes = S::SMEM;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = cs;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    FC_CUDA(cudaLaunchKernelEx(&cfg, kv4_weights_kernel<NB>, c, a, rows, cs, stats));
     FC_LAUNCHED();
     return FC_OK;
 }
@@ -540,16 +604,16 @@ int launch_kv4_prompt(const Kv4& c, const Kv4Attend& a, const KvRows& rows, int 
         default: return launch_prompt_t<8>(c, a, rows, max_rows, stats, device, st);
     }
 }
-int launch_kv4_weights(const Kv4& c, const Kv4Attend& a, const KvRows& rows, const float2* stats, cudaStream_t st) {
+int launch_kv4_weights(const Kv4& c, const Kv4Attend& a, const KvRows& rows, int max_rows, const float2* stats, int device, cudaStream_t st) {
     switch (c.nb) {
-        case 1: return launch_weights_t<1>(c, a, rows, stats, st);
-        case 2: return launch_weights_t<2>(c, a, rows, stats, st);
-        case 3: return launch_weights_t<3>(c, a, rows, stats, st);
-        case 4: return launch_weights_t<4>(c, a, rows, stats, st);
-        case 5: return launch_weights_t<5>(c, a, rows, stats, st);
-        case 6: return launch_weights_t<6>(c, a, rows, stats, st);
-        case 7: return launch_weights_t<7>(c, a, rows, stats, st);
-        default: return launch_weights_t<8>(c, a, rows, stats, st);
+        case 1: return launch_weights_t<1>(c, a, rows, max_rows, stats, device, st);
+        case 2: return launch_weights_t<2>(c, a, rows, max_rows, stats, device, st);
+        case 3: return launch_weights_t<3>(c, a, rows, max_rows, stats, device, st);
+        case 4: return launch_weights_t<4>(c, a, rows, max_rows, stats, device, st);
+        case 5: return launch_weights_t<5>(c, a, rows, max_rows, stats, device, st);
+        case 6: return launch_weights_t<6>(c, a, rows, max_rows, stats, device, st);
+        case 7: return launch_weights_t<7>(c, a, rows, max_rows, stats, device, st);
+        default: return launch_weights_t<8>(c, a, rows, max_rows, stats, device, st);
     }
 }
 

@@ -1,9 +1,12 @@
 // Attention of few query rows over the cache of 4-bit levels (layout: kv4.cuh): decode steps and short drafts.
 //
 // The query rows of a key / value head (rows x heads that share it) are the eight columns of matrix products whose other operand is the
-// cache: S^T = K q^T with levels as they are (exact in f16) and q in two f16 planes, a block's sum times its f16 scale in f32;
-// O^T = V P^T with the weights times the value's scale in two planes. Every sum of products of a tile starts from zero and is added to the
-// row's sums in f32, because the tensor core truncates: what it loses in a tile of 32 positions stays below a rounding of the whole.
+// cache: S^T = K q^T and O^T = V P^T, with levels as they are, exact in f16, and q and P in two f16 planes (22 bits). Up to four
+// columns, both planes lie side by side in one product (SPLIT), whose halves are added afterwards: half the products, and half the
+// weights a lane has to see to. Keys: a block's sum times its scale is added in f32. (Nibbles as f16 subnormals, with -8 times the sum
+// of q to start from, save four instructions a word and cost a digit: 1.8e-6 instead of 2e-7 of the result.) Values: the weight times the
+// value's scale is formed in f16 pairs, rn(ph d) and (ph d - rn(ph d)) + pl d of p = ph + pl. Every sum of products of a tile starts anew and
+// is added to the row's sums in f32, because the tensor core truncates: what it loses in 32 positions stays below a rounding of the whole.
 //
 // A cluster shares a (sequence, head): its warps take tiles of 32 positions in turn, each with a running maximum and sum of its
 // own and its next tiles on the way to shared memory, and join through distributed shared memory at the end: no scratch memory, nothing
@@ -18,10 +21,10 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int SW = 8, COLS = 8, TILE = 32;
+constexpr int COLS = 8, TILE = 32;                // columns of a product, positions a tile
 constexpr int kStepRows = 32;                     // most new rows of a sequence
 
-template <int NB>
+template <int NB, int SW>
 struct StepShape {
     static constexpr int DIM = NB * kKvBlock, PAD = DIM + 4;
     static constexpr int STAGES = NB <= 2 ? 3 : 2;
@@ -29,12 +32,12 @@ struct StepShape {
     static constexpr int RING = SW * STAGES * BYTES;
     static constexpr int FRESH = kStepRows * NB * 36;    // new rows, quantised; then the CTA's joined result
     static constexpr int SMEM = RING + (FRESH > COLS * PAD * 4 ? FRESH : COLS * PAD * 4);
-    static constexpr int CTAS = NB <= 4 ? 2 : 1;
+    static constexpr int CTAS = (NB <= 4 ? 16 : 8) / SW;
 };
 
 template <int NB>
 __device__ __forceinline__ void ask(const Kv4& c, size_t row, char* tile, int lane, bool values) {
-    using S = StepShape<NB>;
+    using S = StepShape<NB, 8>;
     const char *kq = (const char*)(c.kq + row * (NB * 4)), *vq = (const char*)(c.vq + row * (NB * 4));
 #pragma unroll
     for (int i = 0; i < NB; ++i) cp16(tile + i * 512 + lane * 16, kq + i * 512 + lane * 16);
@@ -47,58 +50,97 @@ __device__ __forceinline__ void ask(const Kv4& c, size_t row, char* tile, int la
     }
 }
 
-// The scores of a tile: s[m][0..1]: position 16 m + g, columns 2 t and 2 t + 1; s[m][2..3]: position 16 m + g + 8. -inf behind what a column sees.
-template <int NB>
-__device__ __forceinline__ void tile_scores(const char* tile, const uint32_t (&qh)[NB][4], const uint32_t (&ql)[NB][4], float inv0, float inv1, int j0, int seen0,
-                                            int seen1, int g, int t, float (&s)[2][4]) {
-    using S = StepShape<NB>;
+// What a lane (g, t) has of q: fragments of channels 32 b + 8 t .. + 7 of its column.
+template <int NB, bool SPLIT>
+struct Query {
+    uint32_t f[NB][4];                           // SPLIT: of plane g / 4 of column g % 4; else the high plane of column g
+    uint32_t r[SPLIT ? 1 : NB][4];               // the low plane
+    float inv0, inv1;                            // of this lane's columns of scores
+};
+
+// The scores of a tile. SPLIT: s[m][0..1] are position 16 m + g + 8 (t / 2), columns 2 (t % 2) and + 1. Else s[m][0..1] position 16 m + g,
+// columns 2 t and + 1, s[m][2..3] position 16 m + g + 8. With `edge`, -inf behind what a column sees.
+template <int NB, bool SPLIT>
+__device__ __forceinline__ void tile_scores(const char* tile, const Query<NB, SPLIT>& q, bool edge, int j0, int seen0, int seen1, int g, int t, float (&s)[2][SPLIT ? 2 : 4]) {
+    using S = StepShape<NB, 8>;
     const uint32_t* kq = (const uint32_t*)tile;
     const __half* kd = (const __half*)(tile + 2 * S::KBYTES);
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
         uint32_t w0[NB], w1[NB];
-        float d0[NB], d1[NB];
+        float d0[NB], d1[NB], x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
         const int r = 16 * m + g;
         load_words(kq + r * (NB * 4) + t * NB, w0);
         load_words(kq + (r + 8) * (NB * 4) + t * NB, w1);
         load_scales(kd + r * NB, d0);
         load_scales(kd + (r + 8) * NB, d1);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[m][i] = 0.0f;
-#pragma unroll
         for (int b = 0; b < NB; ++b) {
             uint32_t f0[4], f1[4];
             levels_of(w0[b], f0);
             levels_of(w1[b], f1);
             const uint32_t a0[4] = {f0[0], f1[0], f0[1], f1[1]}, a1[4] = {f0[2], f1[2], f0[3], f1[3]};
-            float x[4] = {0.0f, 0.0f, 0.0f, 0.0f}, y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            mma16816(x, a0, qh[b][0], qh[b][1]);
-            mma16816(y, a0, ql[b][0], ql[b][1]);
-            mma16816(x, a1, qh[b][2], qh[b][3]);
-            mma16816(y, a1, ql[b][2], ql[b][3]);
-            s[m][0] = fmaf(x[0] + y[0], d0[b], s[m][0]);
-            s[m][1] = fmaf(x[1] + y[1], d0[b], s[m][1]);
-            s[m][2] = fmaf(x[2] + y[2], d1[b], s[m][2]);
-            s[m][3] = fmaf(x[3] + y[3], d1[b], s[m][3]);
+            float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            mma16816(y, a0, q.f[b][0], q.f[b][1]);
+            mma16816(y, a1, q.f[b][2], q.f[b][3]);
+            if (!SPLIT) {
+                constexpr int ONE = SPLIT ? 0 : 1;
+                float z[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                mma16816(z, a0, q.r[b * ONE][0], q.r[b * ONE][1]);
+                mma16816(z, a1, q.r[b * ONE][2], q.r[b * ONE][3]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) y[e] += z[e];
+            }
+            x[0] = fmaf(y[0], d0[b], x[0]);
+            x[1] = fmaf(y[1], d0[b], x[1]);
+            x[2] = fmaf(y[2], d1[b], x[2]);
+            x[3] = fmaf(y[3], d1[b], x[3]);
         }
-        s[m][0] = j0 + r < seen0 ? s[m][0] * inv0 : -INFINITY;
-        s[m][1] = j0 + r < seen1 ? s[m][1] * inv1 : -INFINITY;
-        s[m][2] = j0 + r + 8 < seen0 ? s[m][2] * inv0 : -INFINITY;
-        s[m][3] = j0 + r + 8 < seen1 ? s[m][3] * inv1 : -INFINITY;
+        if (SPLIT) {
+            // the planes of a column meet: lanes t < 2 keep position g, the others position g + 8
+            const bool upper = t >= 2;
+            const float y0 = __shfl_xor_sync(0xffffffffu, upper ? x[0] : x[2], 2), y1 = __shfl_xor_sync(0xffffffffu, upper ? x[1] : x[3], 2);
+            s[m][0] = ((upper ? x[2] : x[0]) + y0) * q.inv0;
+            s[m][1] = ((upper ? x[3] : x[1]) + y1) * q.inv1;
+            if (edge) {
+                const int j = j0 + r + 8 * (t >> 1);
+                s[m][0] = j < seen0 ? s[m][0] : -INFINITY;
+                s[m][1] = j < seen1 ? s[m][1] : -INFINITY;
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                s[m][SPLIT ? 0 : e] = x[e] * (e & 1 ? q.inv1 : q.inv0);
+                if (edge) s[m][SPLIT ? 0 : e] = j0 + r + 8 * (e >> 1) < (e & 1 ? seen1 : seen0) ? s[m][SPLIT ? 0 : e] : -INFINITY;
+            }
+        }
     }
 }
 
-template <int NB>
-__global__ void __launch_bounds__(32 * SW, StepShape<NB>::CTAS) kv4_step_kernel(Kv4 c, Kv4Attend a, KvRows rows, float2* __restrict__ stats) {
-    using S = StepShape<NB>;
-    constexpr int DIM = S::DIM, PAD = S::PAD;
+__device__ __forceinline__ uint32_t hmul2u(uint32_t a, uint32_t b) {
+    const __half2 r = __hmul2(*(const __half2*)&a, *(const __half2*)&b);
+    return *(const uint32_t*)&r;
+}
+__device__ __forceinline__ uint32_t hfma2u(uint32_t a, uint32_t b, uint32_t c) {
+    const __half2 r = __hfma2(*(const __half2*)&a, *(const __half2*)&b, *(const __half2*)&c);
+    return *(const uint32_t*)&r;
+}
+__device__ __forceinline__ uint32_t hmax2u(uint32_t a, uint32_t b) {
+    const __half2 r = __hmax2(*(const __half2*)&a, *(const __half2*)&b);
+    return *(const uint32_t*)&r;
+}
+
+template <int NB, bool SPLIT, int SW>
+__global__ void __launch_bounds__(32 * SW, StepShape<NB, SW>::CTAS) kv4_step_kernel(Kv4 c, Kv4Attend a, KvRows rows, float2* __restrict__ stats) {
+    using S = StepShape<NB, SW>;
+    constexpr int DIM = S::DIM, PAD = S::PAD, CALL = SPLIT ? COLS / 2 : COLS;      // columns of a call
     extern __shared__ __align__(16) char smem[];
     __shared__ float2 warp_ml[SW][COLS];          // running maximum (base 2) and sum
     __shared__ float warp_f[SW][COLS];
     __shared__ float2 cta_ml[COLS];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const int cs = gridDim.x, rank = blockIdx.x, h = blockIdx.y % c.n_kv, col0 = blockIdx.y / c.n_kv * COLS, seq = blockIdx.z;
-    const int first = rows.start[seq], n = rows.start[seq + 1] - first, cols = min(n * a.group - col0, COLS);
+    const int cs = gridDim.x, rank = blockIdx.x, h = blockIdx.y % c.n_kv, col0 = blockIdx.y / c.n_kv * CALL, seq = blockIdx.z;
+    const int first = rows.start[seq], n = rows.start[seq + 1] - first, cols = min(n * a.group - col0, CALL);
     if (cols <= 0) return;                        // the whole cluster
     const int len = a.lens[seq], end = a.k ? len + n : len;
     float* const out = a.out + (size_t)first * a.ldo + (size_t)h * a.group * DIM;
@@ -155,20 +197,21 @@ __global__ void __launch_bounds__(32 * SW, StepShape<NB>::CTAS) kv4_step_kernel(
         __syncthreads();
     }
 
-    // column g of this lane's fragments: channels 32 b + 8 t .. + 7 as two planes, brought to [2^13, 2^14) by a power of two
-    uint32_t qh[NB][4], ql[NB][4];
-    float inv;
+    // q: brought to [2^13, 2^14) by a power of two a column
+    const int col = SPLIT ? g & 3 : g, plane = SPLIT ? g >> 2 : 0;
+    const int c0 = SPLIT ? 2 * (t & 1) : 2 * t, c1 = c0 + 1;          // this lane's columns of scores
+    Query<NB, SPLIT> q;
     {
         float x[NB][8];
-        const bool live = g < cols;
-        const int i = (col0 + g) / a.group, head = h * a.group + (col0 + g) - i * a.group;
-        const float* q = a.q + (size_t)(first + i) * a.ldq + (size_t)head * DIM + 8 * t;
+        const bool live = col < cols;
+        const int i = (col0 + col) / a.group, head = h * a.group + (col0 + col) - i * a.group;
+        const float* from = a.q + (size_t)(first + i) * a.ldq + (size_t)head * DIM + 8 * t;
         const float scale = a.scale * 1.44269504f;
         float top = 0.0f;
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-            const float4 lo = live ? *(const float4*)(q + 32 * b) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            const float4 hi = live ? *(const float4*)(q + 32 * b + 4) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            const float4 lo = live ? *(const float4*)(from + 32 * b) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            const float4 hi = live ? *(const float4*)(from + 32 * b + 4) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             const float v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
             for (int j = 0; j < 8; ++j) { x[b][j] = v[j] * scale; top = fmaxf(top, fabsf(x[b][j])); }
@@ -176,22 +219,27 @@ __global__ void __launch_bounds__(32 * SW, StepShape<NB>::CTAS) kv4_step_kernel(
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
         const int shift = plane_shift(top);
-        const float up = exp2i(shift);
-        inv = exp2i(-shift);
+        const float up = exp2i(shift), inv = exp2i(-shift);
+        q.inv0 = __shfl_sync(0xffffffffu, inv, 4 * c0);
+        q.inv1 = __shfl_sync(0xffffffffu, inv, 4 * c1);
 #pragma unroll
         for (int b = 0; b < NB; ++b)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) planes_of(x[b][j] * up, x[b][j + 4] * up, &qh[b][j], &ql[b][j]);
+            for (int j = 0; j < 4; ++j) {
+                uint32_t hi, lo;
+                planes_of(x[b][j] * up, x[b][j + 4] * up, &hi, &lo);
+                q.f[b][j] = SPLIT && plane ? lo : hi;
+                if (!SPLIT) q.r[SPLIT ? 0 : b][j] = lo;
+            }
     }
-    const float inv0 = __shfl_sync(0xffffffffu, inv, 8 * t), inv1 = __shfl_sync(0xffffffffu, inv, 8 * t + 4);
-    const int seen0 = 2 * t < cols ? base + (col0 + 2 * t) / a.group : 0, seen1 = 2 * t + 1 < cols ? base + (col0 + 2 * t + 1) / a.group : 0;
-
-    const int seen_g = g < cols ? base + (col0 + g) / a.group : 0;
+    auto sees = [&](int x) { return x < cols ? base + (col0 + x) / a.group : 0; };
+    const int seen0 = sees(c0), seen1 = sees(c1), seen_g = sees(col);
+    const int whole_tiles = cols == CALL ? max(0, base + col0 / a.group) / TILE : 0;      // that every column sees whole
 
     float o[NB][2][4] = {}, m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
-    float s[2][4];
+    float s[2][SPLIT ? 2 : 4];
     int stage = 0;
-    for (int tile = mine, i = 0; tile < tiles; tile += stride, ++i) {
+    for (int tile = mine; tile < tiles; tile += stride) {
         char* at = ring + stage * S::BYTES;
         {
             const int ahead = tile + (S::STAGES - 1) * stride;
@@ -203,6 +251,7 @@ __global__ void __launch_bounds__(32 * SW, StepShape<NB>::CTAS) kv4_step_kernel(
         cp_wait<S::STAGES - 1>();
         __syncwarp();
         const int j0 = tile * TILE;
+        const bool edge = tile >= whole_tiles;
         if (a.k && j0 + TILE > len) {
             // new rows over what the tile holds of them
             for (int r = max(len - j0, 0); r < TILE && j0 + r < len + n; ++r) {
@@ -217,18 +266,23 @@ __global__ void __launch_bounds__(32 * SW, StepShape<NB>::CTAS) kv4_step_kernel(
             }
             __syncwarp();
         }
-        tile_scores<NB>(at, qh, ql, inv0, inv1, j0, seen0, seen1, g, t, s);
-        float t0 = fmaxf(fmaxf(s[0][0], s[0][2]), fmaxf(s[1][0], s[1][2])), t1 = fmaxf(fmaxf(s[0][1], s[0][3]), fmaxf(s[1][1], s[1][3]));
+        tile_scores<NB, SPLIT>(at, q, edge, j0, seen0, seen1, g, t, s);
+        float t0 = fmaxf(s[0][0], s[1][0]), t1 = fmaxf(s[0][1], s[1][1]);
+        if (!SPLIT) {
+            constexpr int LO = SPLIT ? 0 : 2, HI = SPLIT ? 1 : 3;
+            t0 = fmaxf(t0, fmaxf(s[0][LO], s[1][LO]));
+            t1 = fmaxf(t1, fmaxf(s[0][HI], s[1][HI]));
+        }
 #pragma unroll
-        for (int w = 4; w < 32; w <<= 1) {
+        for (int w = SPLIT ? 2 : 4; w < 32; w <<= 1) {
             t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, w));
             t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, w));
         }
         t0 = fmaxf(t0, m0);
         t1 = fmaxf(t1, m1);
-        const float z0 = t0 == -INFINITY ? 0.0f : t0, z1 = t1 == -INFINITY ? 0.0f : t1;
+        const float z0 = (t0 == -INFINITY ? 0.0f : t0) - kLift, z1 = (t1 == -INFINITY ? 0.0f : t1) - kLift;
         if (__any_sync(0xffffffffu, t0 != m0 || t1 != m1)) {
-            const float f0 = ex2(m0 - z0), f1 = ex2(m1 - z1);
+            const float f0 = ex2(m0 - kLift - z0), f1 = ex2(m1 - kLift - z1);
             l0 *= f0; l1 *= f1;
 #pragma unroll
             for (int b = 0; b < NB; ++b)
@@ -236,43 +290,62 @@ __global__ void __launch_bounds__(32 * SW, StepShape<NB>::CTAS) kv4_step_kernel(
                 for (int u = 0; u < 2; ++u) { o[b][u][0] *= f0; o[b][u][1] *= f1; o[b][u][2] *= f0; o[b][u][3] *= f1; }
             m0 = t0; m1 = t1;
         }
-        // weights, from (position g, columns 2 t, 2 t + 1) to (positions 2 t, 2 t + 1, column g)
-        float p[2][4];
+        // weights as planes, from (position, columns) to (positions 2 t, 2 t + 1 and 2 t + 8, 2 t + 9, column g)
+        uint32_t ph[2][2], pl[2][2];
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const float x = ex2(s[m][2 * u] - z0), y = ex2(s[m][2 * u + 1] - z1);
+            if (SPLIT) {
+                const float x = ex2(s[m][0] - z0), y = ex2(s[m][1] - z1);
                 l0 += x; l1 += y;
                 const uint32_t xb = __float_as_uint(x), yb = __float_as_uint(y);
                 const uint32_t hi = movmatrix(__byte_perm(xb, yb, 0x7632)), lo = movmatrix(__byte_perm(xb, yb, 0x5410));
-                p[m][2 * u] = __uint_as_float(__byte_perm(lo, hi, 0x5410));
-                p[m][2 * u + 1] = __uint_as_float(__byte_perm(lo, hi, 0x7632));
+                // lanes g < 4 have positions 2 t, 2 t + 1 of column g, the others 2 t + 8, 2 t + 9 of column g - 4
+                uint32_t h0, r0;
+                planes_of(__uint_as_float(__byte_perm(lo, hi, 0x5410)), __uint_as_float(__byte_perm(lo, hi, 0x7632)), &h0, &r0);
+                const uint32_t h1 = __shfl_xor_sync(0xffffffffu, h0, 16), r1 = __shfl_xor_sync(0xffffffffu, r0, 16);
+                ph[m][0] = plane ? h1 : h0; ph[m][1] = plane ? h0 : h1;
+                pl[m][0] = plane ? r1 : r0; pl[m][1] = plane ? r0 : r1;
+            } else {
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const float x = ex2(s[m][SPLIT ? 0 : 2 * u] - z0), y = ex2(s[m][SPLIT ? 1 : 2 * u + 1] - z1);
+                    l0 += x; l1 += y;
+                    const uint32_t xb = __float_as_uint(x), yb = __float_as_uint(y);
+                    const uint32_t hi = movmatrix(__byte_perm(xb, yb, 0x7632)), lo = movmatrix(__byte_perm(xb, yb, 0x5410));
+                    planes_of(__uint_as_float(__byte_perm(lo, hi, 0x5410)), __uint_as_float(__byte_perm(lo, hi, 0x7632)), &ph[m][u], &pl[m][u]);
+                }
             }
         }
-        // scales of the values, and the power of two that brings the largest product of the tile into [2^13, 2^14): of what column g sees,
-        // as what lies behind must not change a bit
-        const bool edge = j0 + TILE > base + col0 / a.group;
+        // scales of the values in pairs of positions, times a power of two that brings the largest of the tile to 2^kScaleLift and above
+        // (2^15 at most): the largest that column g sees, as what lies behind must not change a bit
         const __half* vd = (const __half*)(at + 2 * S::KBYTES + S::DBYTES);
-        float d[2][4][NB], top = 0.0f;
+        uint32_t d[2][2][NB], most = 0;
 #pragma unroll
         for (int m = 0; m < 2; ++m)
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                load_scales(vd + (16 * m + 2 * t + (u & 1) + 8 * (u >> 1)) * NB, d[m][u]);
-                const bool out_of_sight = edge && j0 + 16 * m + 2 * t + (u & 1) + 8 * (u >> 1) >= seen_g;
+            for (int u = 0; u < 2; ++u) {
+                uint32_t w[NB];                   // the scales of two positions, one after the other
+                load_words((const uint32_t*)(vd + (16 * m + 2 * t + 8 * u) * NB), w);
 #pragma unroll
-                for (int b = 0; b < NB; ++b) top = fmaxf(top, out_of_sight ? 0.0f : fabsf(d[m][u][b]));
+                for (int b = 0; b < NB; ++b) {
+                    const int x = b, y = NB + b;  // halves of w
+                    d[m][u][b] = __byte_perm(w[x >> 1], w[y >> 1], (x & 1 ? 0x32 : 0x10) | (y & 1 ? 0x7600 : 0x5400));
+                }
+                if (edge) {                       // what a weight of 0 meets is 0: what lies there could be large
+                    const int j = j0 + 16 * m + 2 * t + 8 * u;
+                    const uint32_t sight = (j < seen_g ? 0xffffu : 0u) | (j + 1 < seen_g ? 0xffff0000u : 0u);
+#pragma unroll
+                    for (int b = 0; b < NB; ++b) d[m][u][b] &= sight;
+                }
+#pragma unroll
+                for (int b = 0; b < NB; ++b) most = hmax2u(most, d[m][u][b] & 0x7fff7fffu);
             }
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const int shift = plane_shift(top);
-        const float up = exp2i(shift), down = exp2i(-shift);
-        const float down0 = edge ? __shfl_sync(0xffffffffu, down, 8 * t) : down, down1 = edge ? __shfl_sync(0xffffffffu, down, 8 * t + 4) : down;
-#pragma unroll
-        for (int m = 0; m < 2; ++m)
-#pragma unroll
-            for (int u = 0; u < 4; ++u) p[m][u] *= up;
+        most = hmax2u(most, __shfl_xor_sync(0xffffffffu, most, 1));
+        most = hmax2u(most, __shfl_xor_sync(0xffffffffu, most, 2));
+        const int exponent = (int)(max(most & 0xffffu, most >> 16) >> 10), lift = min(15 + kScaleLift - exponent, 15);
+        const uint32_t by = (uint32_t)(15 + lift) << 10;      // 2^lift, -8 <= lift
+        const uint32_t up = by | by << 16;
+        const float down = exp2i(-lift), down0 = edge ? __shfl_sync(0xffffffffu, down, 4 * c0) : down, down1 = edge ? __shfl_sync(0xffffffffu, down, 4 * c1) : down;
         const uint32_t* vq = (const uint32_t*)(at + S::KBYTES);
         uint32_t w[4][NB];                        // pairs of positions t, t + 4, t + 8, t + 12
 #pragma unroll
@@ -282,16 +355,21 @@ __global__ void __launch_bounds__(32 * SW, StepShape<NB>::CTAS) kv4_step_kernel(
             float x[2][4] = {};
 #pragma unroll
             for (int m = 0; m < 2; ++m) {
-                uint32_t h0, h1, r0, r1, e0[4], e1[4];
-                planes_of(p[m][0] * d[m][0][b], p[m][1] * d[m][1][b], &h0, &r0);
-                planes_of(p[m][2] * d[m][2][b], p[m][3] * d[m][3][b], &h1, &r1);
+                uint32_t hi[2], lo[2], e0[4], e1[4];
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const uint32_t f = hmul2u(d[m][u][b], up);
+                    hi[u] = hmul2u(ph[m][u], f);
+                    lo[u] = hfma2u(pl[m][u], f, hfma2u(ph[m][u], f, hi[u] ^ 0x80008000u));
+                    if (SPLIT) hi[u] = plane ? lo[u] : hi[u];
+                }
                 levels_of(w[2 * m][b], e0);
                 levels_of(w[2 * m + 1][b], e1);
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
                     const uint32_t f[4] = {e0[2 * u], e0[2 * u + 1], e1[2 * u], e1[2 * u + 1]};
-                    mma16816(x[u], f, r0, r1);
-                    mma16816(x[u], f, h0, h1);
+                    if (!SPLIT) mma16816(x[u], f, lo[0], lo[1]);
+                    mma16816(x[u], f, hi[0], hi[1]);
                 }
             }
 #pragma unroll
@@ -304,97 +382,127 @@ __global__ void __launch_bounds__(32 * SW, StepShape<NB>::CTAS) kv4_step_kernel(
     cp_wait<0>();
     __syncwarp();
 #pragma unroll
-    for (int w = 4; w < 32; w <<= 1) {
+    for (int w = SPLIT ? 2 : 4; w < 32; w <<= 1) {
         l0 += __shfl_xor_sync(0xffffffffu, l0, w);
         l1 += __shfl_xor_sync(0xffffffffu, l1, w);
     }
-    if (g == 0) {
-        warp_ml[warp][2 * t] = make_float2(m0, l0);
-        warp_ml[warp][2 * t + 1] = make_float2(m1, l1);
+    if (g == 0 && (!SPLIT || t < 2)) {
+        warp_ml[warp][c0] = make_float2(m0, l0);
+        warp_ml[warp][c1] = make_float2(m1, l1);
     }
     float* const mo = (float*)ring;               // [column][channel]
+    if (SPLIT) {
+        // the planes of a weight meet: lanes t < 2 keep channels g, the others channels g + 8
 #pragma unroll
-    for (int b = 0; b < NB; ++b)
+        for (int b = 0; b < NB; ++b)
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const int ch = 32 * b + 16 * u + g;
-            mo[2 * t * PAD + ch] = o[b][u][0];
-            mo[(2 * t + 1) * PAD + ch] = o[b][u][1];
-            mo[2 * t * PAD + ch + 8] = o[b][u][2];
-            mo[(2 * t + 1) * PAD + ch + 8] = o[b][u][3];
-        }
+            for (int u = 0; u < 2; ++u) {
+                const bool upper = t >= 2;
+                const float y0 = __shfl_xor_sync(0xffffffffu, upper ? o[b][u][0] : o[b][u][2], 2), y1 = __shfl_xor_sync(0xffffffffu, upper ? o[b][u][1] : o[b][u][3], 2);
+                const int ch = 32 * b + 16 * u + g + (upper ? 8 : 0);
+                mo[c0 * PAD + ch] = (upper ? o[b][u][2] : o[b][u][0]) + y0;
+                mo[c1 * PAD + ch] = (upper ? o[b][u][3] : o[b][u][1]) + y1;
+            }
+    } else {
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int ch = 32 * b + 16 * u + g;
+                mo[c0 * PAD + ch] = o[b][u][0];
+                mo[c1 * PAD + ch] = o[b][u][1];
+                mo[c0 * PAD + ch + 8] = o[b][u][2];
+                mo[c1 * PAD + ch + 8] = o[b][u][3];
+            }
+    }
     __syncthreads();
-    if (tid < SW * COLS) {
-        const int col = tid % COLS;
+    if (tid < SW * CALL) {
+        const int x = tid % CALL;
         float m = -INFINITY, l = 0.0f;
 #pragma unroll
-        for (int w = 0; w < SW; ++w) m = fmaxf(m, warp_ml[w][col].x);
+        for (int w = 0; w < SW; ++w) m = fmaxf(m, warp_ml[w][x].x);
         const float z = m == -INFINITY ? 0.0f : m;
 #pragma unroll
-        for (int w = 0; w < SW; ++w) l += warp_ml[w][col].y * ex2(warp_ml[w][col].x - z);
-        warp_f[tid / COLS][col] = ex2(warp_ml[tid / COLS][col].x - z);
-        if (tid < COLS) cta_ml[col] = make_float2(m, l);
+        for (int w = 0; w < SW; ++w) l += warp_ml[w][x].y * ex2(warp_ml[w][x].x - z);
+        warp_f[tid / CALL][x] = ex2(warp_ml[tid / CALL][x].x - z);
+        if (tid < CALL) cta_ml[x] = make_float2(m, l);
     }
     __syncthreads();
     float* const joined = (float*)fresh;          // the new rows in it have been read
-    for (int e = tid; e < COLS * DIM; e += 32 * SW) {
-        const int col = e / DIM, ch = e % DIM;
-        float x = 0.0f;
+    for (int e = tid; e < CALL * DIM; e += 32 * SW) {
+        const int x = e / DIM, ch = e % DIM;
+        float y = 0.0f;
 #pragma unroll
-        for (int w = 0; w < SW; ++w) x = fmaf(((const float*)(smem + w * (S::STAGES * S::BYTES)))[col * PAD + ch], warp_f[w][col], x);
-        joined[col * PAD + ch] = x;
+        for (int w = 0; w < SW; ++w) y = fmaf(((const float*)(smem + w * (S::STAGES * S::BYTES)))[x * PAD + ch], warp_f[w][x], y);
+        if (cs == 1) {
+            if (x < cols) out[place(x) + ch] = cta_ml[x].y == 0.0f ? 0.0f : y / cta_ml[x].y;
+        } else {
+            joined[x * PAD + ch] = y;
+        }
     }
     cg::cluster_group cluster = cg::this_cluster();
     if (cs > 1) cluster.sync();
-    else __syncthreads();
-    // every rank joins its share of the elements
-    auto whole = [&](int col, float* z) {
+    // a column's maximum and sum over the ranks
+    auto whole = [&](int x, float* z) {
         float m = -INFINITY, l = 0.0f;
-        for (int r = 0; r < cs; ++r) m = fmaxf(m, cluster.map_shared_rank(cta_ml, r)[col].x);
+        for (int r = 0; r < cs; ++r) m = fmaxf(m, cluster.map_shared_rank(cta_ml, r)[x].x);
         *z = m == -INFINITY ? 0.0f : m;
         for (int r = 0; r < cs; ++r) {
-            const float2 x = cluster.map_shared_rank(cta_ml, r)[col];
-            l = fmaf(x.y, ex2(x.x - *z), l);
+            const float2 y = cluster.map_shared_rank(cta_ml, r)[x];
+            l = fmaf(y.y, ex2(y.x - *z), l);
         }
         return l;
     };
-    for (int e = rank * (32 * SW) + tid; e < cols * DIM; e += cs * (32 * SW)) {
-        const int col = e / DIM, ch = e % DIM;
-        float z, x = 0.0f;
-        const float l = whole(col, &z);
-        for (int r = 0; r < cs; ++r) x = fmaf(cluster.map_shared_rank(joined, r)[col * PAD + ch], ex2(cluster.map_shared_rank(cta_ml, r)[col].x - z), x);
-        out[place(col) + ch] = l == 0.0f ? 0.0f : x / l;
-        if (ch == 0 && stats) stats[((size_t)first + (col0 + col) / a.group) * (c.n_kv * a.group) + h * a.group + (col0 + col) % a.group] = make_float2(z, l);
+    // every rank joins its share of the elements
+    for (int e = rank * (32 * SW) + tid; cs > 1 && e < cols * DIM; e += cs * (32 * SW)) {
+        const int x = e / DIM, ch = e % DIM;
+        float z, y = 0.0f;
+        const float l = whole(x, &z);
+        for (int r = 0; r < cs; ++r) y = fmaf(cluster.map_shared_rank(joined, r)[x * PAD + ch], ex2(cluster.map_shared_rank(cta_ml, r)[x].x - z), y);
+        out[place(x) + ch] = l == 0.0f ? 0.0f : y / l;
+    }
+    if (stats && rank == 0 && tid < cols) {
+        float z;
+        const float l = whole(tid, &z);
+        stats[((size_t)first + (col0 + tid) / a.group) * (c.n_kv * a.group) + h * a.group + (col0 + tid) % a.group] = make_float2(z - kLift, l);
     }
     if (a.mass && !stats) {
         // the weights once more, against the whole row's maximum and sum: the last tile's scores are still there
         float z0, z1;
-        l0 = whole(2 * t, &z0);
-        l1 = whole(2 * t + 1, &z1);
-        l0 = 2 * t < cols && l0 != 0.0f ? 1.0f / l0 : 0.0f;
-        l1 = 2 * t + 1 < cols && l1 != 0.0f ? 1.0f / l1 : 0.0f;
+        l0 = whole(c0, &z0);
+        l1 = whole(c1, &z1);
+        l0 = c0 < cols && l0 != 0.0f ? 1.0f / l0 : 0.0f;
+        l1 = c1 < cols && l1 != 0.0f ? 1.0f / l1 : 0.0f;
+        z0 -= kLift; z1 -= kLift;
         float* const mass = a.mass + ((size_t)seq * c.n_kv + h) * c.cap;
         if (cs > 1) cluster.sync();               // the ring may be written, and no rank leaves while it is read
         else __syncthreads();
         const int last = tiles > mine ? mine + (tiles - 1 - mine) / stride * stride : -1;
+#pragma unroll
+        for (int i = 1; i < S::STAGES; ++i) {
+            if (last - i * stride >= 0) ask<NB>(c, row0 + (size_t)(last - i * stride) * TILE, ring + i * S::BYTES, lane, false);
+            cp_commit();
+        }
+        stage = 0;
         for (int tile = last; tile >= 0; tile -= stride) {
             if (tile != last) {
+                cp_wait<S::STAGES - 2>();
                 __syncwarp();
-                ask<NB>(c, row0 + (size_t)tile * TILE, ring, lane, false);
-                cp_commit();
-                cp_wait<0>();
+                tile_scores<NB, SPLIT>(ring + stage * S::BYTES, q, true, tile * TILE, seen0, seen1, g, t, s);
                 __syncwarp();
-                tile_scores<NB>(ring, qh, ql, inv0, inv1, tile * TILE, seen0, seen1, g, t, s);
             }
+            if (tile - S::STAGES * stride >= 0) ask<NB>(c, row0 + (size_t)(tile - S::STAGES * stride) * TILE, ring + stage * S::BYTES, lane, false);
+            cp_commit();
+            stage = stage + 1 == S::STAGES ? 0 : stage + 1;
 #pragma unroll
             for (int m = 0; m < 2; ++m)
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
+                for (int u = 0; u < (SPLIT ? 1 : 2); ++u) {
                     float x = (l0 != 0.0f ? ex2(s[m][2 * u] - z0) * l0 : 0.0f) + (l1 != 0.0f ? ex2(s[m][2 * u + 1] - z1) * l1 : 0.0f);
                     x += __shfl_xor_sync(0xffffffffu, x, 1);
-                    x += __shfl_xor_sync(0xffffffffu, x, 2);
-                    const int j = tile * TILE + 16 * m + 8 * u + g;
-                    if (t == 0 && j < end) mass[j] = (j < (a.k ? len : end) ? mass[j] : 0.0f) + x;
+                    if (!SPLIT) x += __shfl_xor_sync(0xffffffffu, x, 2);
+                    const int j = tile * TILE + 16 * m + g + 8 * (SPLIT ? t >> 1 : u);
+                    if ((SPLIT ? t & 1 : t) == 0 && j < end) mass[j] = (j < (a.k ? len : end) ? mass[j] : 0.0f) + x;
                 }
         }
         return;
@@ -402,14 +510,20 @@ __global__ void __launch_bounds__(32 * SW, StepShape<NB>::CTAS) kv4_step_kernel(
     if (cs > 1) cluster.sync();                   // no rank leaves while another reads its memory
 }
 
-template <int NB>
-int launch_step_t(const Kv4& c, const Kv4Attend& a, const KvRows& rows, int groups, int cs, float2* stats, int device, cudaStream_t st) {
-    using S = StepShape<NB>;
+template <int NB, bool SPLIT, int SW>
+int launch_step_t(const Kv4& c, const Kv4Attend& a, const KvRows& rows, int groups, float2* stats, int device, cudaStream_t st) {
+    using S = StepShape<NB, SW>;
+    const auto kernel = kv4_step_kernel<NB, SPLIT, SW>;
     static bool attr_set[64] = {};
     if (device >= 64 || !attr_set[device]) {
-        FC_CUDA(cudaFuncSetAttribute(kv4_step_kernel<NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM));
+        FC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM));
         if (device < 64) attr_set[device] = true;
     }
+    // as many CTAs as are resident, and no more than a tile for each warp of them
+    const long long clusters = (long long)c.n_seq * c.n_kv * groups;
+    const int most = (c.cap + TILE * SW - 1) / (TILE * SW);
+    int cs = 1;
+    while (cs < 8 && cs * 2 <= most && clusters * cs * 2 <= 148 * S::CTAS) cs *= 2;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(cs, c.n_kv * groups, c.n_seq);
     cfg.blockDim = dim3(32 * SW);
@@ -421,9 +535,18 @@ int launch_step_t(const Kv4& c, const Kv4Attend& a, const KvRows& rows, int grou
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    FC_CUDA(cudaLaunchKernelEx(&cfg, kv4_step_kernel<NB>, c, a, rows, stats));
+    FC_CUDA(cudaLaunchKernelEx(&cfg, kernel, c, a, rows, stats));
     FC_LAUNCHED();
     return FC_OK;
+}
+
+template <int NB>
+int launch_step_nb(const Kv4& c, const Kv4Attend& a, const KvRows& rows, int cols, float2* stats, int device, cudaStream_t st) {
+    const bool split = cols <= COLS / 2;
+    const int groups = split ? 1 : (cols + COLS - 1) / COLS;
+    const bool many = (long long)c.n_seq * c.n_kv * groups > 148;
+    if (split) return many ? launch_step_t<NB, true, 4>(c, a, rows, groups, stats, device, st) : launch_step_t<NB, true, 8>(c, a, rows, groups, stats, device, st);
+    return many ? launch_step_t<NB, false, 4>(c, a, rows, groups, stats, device, st) : launch_step_t<NB, false, 8>(c, a, rows, groups, stats, device, st);
 }
 
 }  // namespace
@@ -433,21 +556,16 @@ bool kv4_step_covers(const Kv4& c, int group, int max_rows) {
 }
 
 int launch_kv4_step(const Kv4& c, const Kv4Attend& a, const KvRows& rows, int max_rows, float2* stats, int device, cudaStream_t st) {
-    const int groups = (max_rows * a.group + COLS - 1) / COLS;
-    // as many CTAs as are resident, and no more than a tile for each warp of them
-    const long long clusters = (long long)c.n_seq * c.n_kv * groups;
-    const int most = (c.cap + TILE * SW - 1) / (TILE * SW);
-    int cs = 1;
-    while (cs < 8 && cs * 2 <= most && clusters * cs * 2 <= 296) cs *= 2;
+    const int cols = max_rows * a.group;
     switch (c.nb) {
-        case 1: return launch_step_t<1>(c, a, rows, groups, cs, stats, device, st);
-        case 2: return launch_step_t<2>(c, a, rows, groups, cs, stats, device, st);
-        case 3: return launch_step_t<3>(c, a, rows, groups, cs, stats, device, st);
-        case 4: return launch_step_t<4>(c, a, rows, groups, cs, stats, device, st);
-        case 5: return launch_step_t<5>(c, a, rows, groups, cs, stats, device, st);
-        case 6: return launch_step_t<6>(c, a, rows, groups, cs, stats, device, st);
-        case 7: return launch_step_t<7>(c, a, rows, groups, cs, stats, device, st);
-        default: return launch_step_t<8>(c, a, rows, groups, cs, stats, device, st);
+        case 1: return launch_step_nb<1>(c, a, rows, cols, stats, device, st);
+        case 2: return launch_step_nb<2>(c, a, rows, cols, stats, device, st);
+        case 3: return launch_step_nb<3>(c, a, rows, cols, stats, device, st);
+        case 4: return launch_step_nb<4>(c, a, rows, cols, stats, device, st);
+        case 5: return launch_step_nb<5>(c, a, rows, cols, stats, device, st);
+        case 6: return launch_step_nb<6>(c, a, rows, cols, stats, device, st);
+        case 7: return launch_step_nb<7>(c, a, rows, cols, stats, device, st);
+        default: return launch_step_nb<8>(c, a, rows, cols, stats, device, st);
     }
 }
 

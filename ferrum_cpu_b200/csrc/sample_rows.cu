@@ -57,36 +57,27 @@ struct Row {
 
 struct Weigher {
     double best, scale;                       // log2(e) / T
+    float least;                              // logits below it weigh nothing: 2^-45 at most
     const double* table;
     __device__ __forceinline__ double log2w(float l) const { return ((double)l - best) * scale; }
-    // 2^x for x <= 0 as v 2^n, v in [0.95, 2): x = (16 n + i) / 16 + r, |r| <= 1 / 32
-    __device__ __forceinline__ double part(double x, int* n) const {
+    // 2^(x + up) for -1000 <= x <= 0: x = (16 n + i) / 16 + r, |r| <= 1 / 32
+    __device__ __forceinline__ double power(double x, int up) const {
         const double magic = 6755399441055744.0 / 16.0;      // 1.5 * 2^52 / 16: the sum's last bits are 16 x, rounded
-        const double t = fma(1.0, x, magic);
+        const double t = x + magic;
         const int k = __double2loint(t);
         const double r = x - (t - magic);
         double y = fma(r, 1.3333558146428443e-3, 9.6181291076284772e-3);
         y = fma(r, y, 5.5504108664821580e-2);
         y = fma(r, y, 2.4022650695910071e-1);
         y = fma(r, y, 6.9314718055994531e-1);
-        y = fma(r, y, 1.0);
-        *n = k >> 4;
-        return y * table[k & 15];
+        y = fma(r, y, 1.0) * table[k & 15];                  // in [0.97, 2)
+        return __hiloint2double(__double2hiint(y) + ((k >> 4) + up) * (1 << 20), __double2loint(y));
     }
+    // the sum's last bits are the weight in units of 2^-42, rounded
     __device__ __forceinline__ u64 fixed(double x) const {
-        if (!(x >= -44.0)) return 0;          // less than a quarter of a unit
-        int n;
-        const double v = part(x, &n);
-        // the sum's last bits are v 2^42, rounded
-        const u64 m = (u64)__double_as_longlong(v + 1024.0) & 0xfffffffffffffull;
-        return n == 0 ? m : (m + (1ull << (-n - 1))) >> -n;
+        return (u64)__double_as_longlong(power(x, kFix) + 4503599627370496.0) & 0xfffffffffffffull;
     }
-    __device__ __forceinline__ double exact(double x) const {
-        if (!(x >= -1000.0)) return 0.0;
-        int n;
-        const double v = part(x, &n);
-        return v * __longlong_as_double((long long)(n + 1023) << 52);
-    }
+    __device__ __forceinline__ double exact(double x) const { return power(x, 0); }
 };
 
 __device__ __forceinline__ u64 warp_sum(u64 v) {
@@ -200,7 +191,8 @@ __global__ void __launch_bounds__(RT, 2) sample_rows_kernel(const float* __restr
     if (row.endless) { top = low = 0.0f; }
 
     const double temp = fmax((double)p.temperature, 0.01);
-    const Weigher weigh = {(double)top, 1.4426950408889634 / temp, s.table};
+    // (45 / log2(e) = 31.2; a rounding of the product or the difference does not reach 2^-43)
+    const Weigher weigh = {(double)top, 1.4426950408889634 / temp, top - 31.25f * (float)fmin(temp, 1e30), s.table};
     const bool cut_k = p.top_k > 0 && p.top_k < V, cut_p = p.top_p < 1.0f;
     const double floor_x = p.min_p > 0.0f ? fmax(log2(fmin((double)p.min_p, 1.0)), kLeast) : kLeast;
     // buckets of even width from the largest down to what has a weight
@@ -213,7 +205,7 @@ __global__ void __launch_bounds__(RT, 2) sample_rows_kernel(const float* __restr
         const Weigher& weigh;
         const decltype(bucket_of)& bucket;
         double floor_x;
-        bool by_value, mass_too;
+        bool by_value, count_too, mass_too;
         int lane;
         u64& sum;
         u64& all;
@@ -221,18 +213,19 @@ __global__ void __launch_bounds__(RT, 2) sample_rows_kernel(const float* __restr
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 if (v[e] == -INFINITY) continue;
-                const double x = weigh.log2w(v[e]);
+                const bool weighs = v[e] >= weigh.least;
                 if (by_value) {
-                    const u64 w = mass_too ? weigh.fixed(x) : 0;
+                    const u64 w = mass_too && weighs ? weigh.fixed(weigh.log2w(v[e])) : 0;
                     const int b = bucket(v[e]);
-                    atomicAdd(&s.cnt[b], 1u);
+                    if (count_too) atomicAdd(&s.cnt[b], 1u);
                     if (w) {
                         const unsigned lo = (unsigned)w, old = atomicAdd(&s.lo[b], lo);
                         const unsigned hi = (unsigned)(w >> 32) + (old + lo < lo);
                         if (hi) atomicAdd(&s.hi[b], hi);
                     }
-                } else if (x >= floor_x) {
-                    sum += weigh.fixed(x);
+                } else if (weighs) {
+                    const double x = weigh.log2w(v[e]);
+                    if (x >= floor_x) sum += weigh.fixed(x);
                 }
             }
         }
@@ -246,7 +239,7 @@ __global__ void __launch_bounds__(RT, 2) sample_rows_kernel(const float* __restr
     };
     u64 lane_sum = 0, warp_all = 0;
     const bool by_value = cut_k || cut_p;
-    over(row, begin, end, chunk, Weigh{s, weigh, bucket_of, floor_x, by_value, cut_p, lane, lane_sum, warp_all});
+    over(row, begin, end, chunk, Weigh{s, weigh, bucket_of, floor_x, by_value, cut_k, cut_p, lane, lane_sum, warp_all});
     unsigned cut = 0;
     if (by_value) {
         sync();
@@ -311,7 +304,8 @@ __global__ void __launch_bounds__(RT, 2) sample_rows_kernel(const float* __restr
             const unsigned above_n = s.above_n;
             const u64 above_w = s.above_w;
             auto enough = [&](unsigned k, u64 m) { return ((wants & 1) && above_n + k >= (unsigned)p.top_k) || ((wants & 2) && reached(above_w + m)); };
-            if (s.all_cnt[bucket] <= LIST) {
+            bool listed = !cut_k || s.all_cnt[bucket] <= LIST;
+            if (listed) {
                 struct Gather {
                     Shared& s;
                     const Weigher& weigh;
@@ -325,15 +319,17 @@ __global__ void __launch_bounds__(RT, 2) sample_rows_kernel(const float* __restr
                         for (int e = 0; e < 4; ++e)
                             if (v[e] > -INFINITY && bucket(v[e]) == which) {
                                 const int q = atomicAdd(listed, 1);
+                                if (q >= LIST) continue;
                                 keys[q] = logit_key(v[e]);
-                                ws[q] = weigh.fixed(weigh.log2w(v[e]));
+                                ws[q] = v[e] >= weigh.least ? weigh.fixed(weigh.log2w(v[e])) : 0;
                             }
                     }
                     __device__ void done(int) const {}
                 };
                 over(row, begin, end, chunk, Gather{s, weigh, bucket_of, at(&s.listed, 0), at(s.list_key, 0), at(s.list_w, 0), bucket});
                 sync();
-                if (rank == 0) {
+                listed = *at(&s.listed, 0) <= LIST;
+                if (rank == 0 && listed) {
                     const int n = s.listed;
                     for (int i = tid; i < n; i += RT) {
                         const unsigned key = s.list_key[i];
@@ -350,8 +346,9 @@ __global__ void __launch_bounds__(RT, 2) sample_rows_kernel(const float* __restr
                     }
                 }
                 sync();
-                cut = s.cut;
-            } else {
+                cut = listed ? s.cut : 0;
+            }
+            if (!listed) {
                 // more of them than the list holds: the cut's bits from the highest down, a pass each
                 struct Count {
                     Shared& s;
@@ -367,7 +364,7 @@ __global__ void __launch_bounds__(RT, 2) sample_rows_kernel(const float* __restr
                         for (int e = 0; e < 4; ++e)
                             if (v[e] > -INFINITY && logit_key(v[e]) >= cand && bucket(v[e]) == which) {
                                 ++n;
-                                if (mass_too) w += weigh.fixed(weigh.log2w(v[e]));
+                                if (mass_too && v[e] >= weigh.least) w += weigh.fixed(weigh.log2w(v[e]));
                             }
                     }
                     __device__ void done(int) const {}
@@ -405,7 +402,7 @@ __global__ void __launch_bounds__(RT, 2) sample_rows_kernel(const float* __restr
             __device__ void operator()(const float (&v)[4], int, int) const {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    if (v[e] == -INFINITY || logit_key(v[e]) < cut) continue;
+                    if (!(v[e] >= weigh.least) || logit_key(v[e]) < cut) continue;
                     const double x = weigh.log2w(v[e]);
                     if (x >= floor_x) sum += weigh.fixed(x);
                 }
@@ -463,7 +460,7 @@ __global__ void __launch_bounds__(RT, 2) sample_rows_kernel(const float* __restr
         const int per_lane = chunk / 32, i0 = begin + c0 * chunk + lane * per_lane, i1 = min(i0 + per_lane, end);
         auto weight = [&](int i) -> u64 {
             const float l = row.fix(__ldg(row.p + i));
-            if (l == -INFINITY || logit_key(l) < cut) return 0;
+            if (!(l >= weigh.least) || logit_key(l) < cut) return 0;
             const double x = weigh.log2w(l);
             return x >= floor_x ? weigh.fixed(x) : 0;
         };
