@@ -42,12 +42,19 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(Kv4 c, const float* __r
 // writes eight channels of a row, of keys from one word, of values from the nibble j of eight half words. Bound: the bytes written.
 __global__ void __launch_bounds__(256) kv4_read_kernel(Kv4 c, const int* __restrict__ from, int n, float* __restrict__ k, float* __restrict__ v) {
     const int parts = c.nb * 4, seq = blockIdx.y, base = from ? from[seq] : 0;
-    const size_t all = (size_t)n * c.n_kv * parts;
-    for (size_t e = (size_t)blockIdx.x * blockDim.x + threadIdx.x; e < 2 * all; e += (size_t)gridDim.x * blockDim.x) {
-        const bool values = e >= all;
-        const size_t at = values ? e - all : e;
-        const int part = (int)(at % parts), b = part >> 2, t = part & 3, h = (int)(at / parts % c.n_kv), i = (int)(at / parts / c.n_kv);
-        const long long pos = (long long)base + i;
+    const int per = 128 / parts, e = threadIdx.x & 127, part = e % parts, b = part >> 2, t = part & 3;      // rows a block: half of it keys, half values
+    const bool values = threadIdx.x >= 128;
+    if (e >= per * parts) return;
+    // rows of all heads in the order in which they are written
+    const unsigned first = blockIdx.x * per + e / parts, stride = gridDim.x * per, step_i = stride / (unsigned)c.n_kv, step_h = stride % (unsigned)c.n_kv;
+    long long i = first / (unsigned)c.n_kv;
+    int h = (int)(first % (unsigned)c.n_kv);
+    for (; i < n; i += step_i, h += step_h) {
+        if (h >= c.n_kv) {
+            h -= c.n_kv;
+            if (++i >= n) break;
+        }
+        const long long pos = base + i;
         float x[8] = {};
         if (pos >= 0 && pos < c.cap) {
             const size_t row = c.row(seq, h, (int)pos);
@@ -63,7 +70,7 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(Kv4 c, const int* __restr
                 for (int g = 0; g < 8; ++g) x[g] = d * (float)((int)(w >> (4 * g) & 15) - 8);
             }
         }
-        float4* to = (float4*)((values ? v : k) + ((size_t)seq * all + at) * 8);
+        float4* to = (float4*)((values ? v : k) + ((((size_t)seq * n + i) * c.n_kv + h) * parts + part) * 8);
         to[0] = make_float4(x[0], x[1], x[2], x[3]);
         to[1] = make_float4(x[4], x[5], x[6], x[7]);
     }
@@ -77,12 +84,12 @@ __device__ __forceinline__ unsigned weight_key(float w) {
 }
 
 constexpr int ET = 512, BINS = 2048, KEYS = 16384, LISTED = 2048;
-struct EvictShared {
+struct __align__(16) EvictShared {
     unsigned key[KEYS];
     unsigned bins[BINS];
     int src[LISTED];                               // where the rows of a window of dst come from
     int warp_n[ET / 32], warp_t[ET / 32];
-    int digit, above;
+    int digit, above, in_bin, listed;
 };
 
 // What stays of a (sequence, head), shared by gridDim.x CTAs. Each finds the key of the last position that stays for itself (three passes
@@ -107,19 +114,42 @@ __global__ void __launch_bounds__(ET, 2) kv4_evict_kernel(Kv4 src, Kv4 dst, cons
     const int old = all ? 0 : len - recent, want = budget - recent;      // of the first `old` positions the `want` heaviest
     const bool fits = old <= KEYS;
     if (fits)
-        for (int j = tid; j < old; j += ET) s.key[j] = weight_key(m[j]);
+#pragma unroll 4
+        for (int j = tid; j < old; j += ET) s.key[j] = weight_key(__ldg(m + j));
     auto key = [&](int j) { return fits ? s.key[j] : weight_key(__ldg(m + j)); };
     unsigned cut = 0;
     int ties = want;                               // how many of those at the cut stay, the first ones
     if (!all && want > 0) {
-        int shift = 21, width = 11;
+        int shift = 21, width = 11, listed = 0;
+        unsigned* const list = (unsigned*)s.src;
         for (int pass = 0; pass < 3; ++pass) {
             for (int b = tid; b < BINS; b += ET) s.bins[b] = 0;
+            if (tid == 0) s.listed = 0;
             __syncthreads();
-            const unsigned high = pass ? cut >> (shift + width) : 0;
-            for (int j = tid; j < old; j += ET) {
-                const unsigned k = key(j);
-                if (pass == 0 || k >> (shift + width) == high) atomicAdd(&s.bins[k >> shift & ((1u << width) - 1)], 1u);
+            const unsigned high = pass ? cut >> (shift + width) : 0, mask = (1u << width) - 1;
+            if (pass == 0) {
+#pragma unroll 4
+                for (int j = tid; j < old; j += ET) atomicAdd(&s.bins[key(j) >> shift], 1u);
+            } else if (pass == 1) {
+                // the keys of the first digit's bin, listed where they fit
+                const bool list_them = s.in_bin <= LISTED;
+#pragma unroll 4
+                for (int j = tid; j < old; j += ET) {
+                    const unsigned k = key(j);
+                    if (k >> (shift + width) != high) continue;
+                    atomicAdd(&s.bins[k >> shift & mask], 1u);
+                    if (list_them) list[atomicAdd(&s.listed, 1)] = k;
+                }
+                listed = list_them;
+            } else if (listed) {
+                for (int j = tid; j < s.in_bin; j += ET)
+                    if (list[j] >> (shift + width) == high) atomicAdd(&s.bins[list[j] >> shift & mask], 1u);
+            } else {
+#pragma unroll 4
+                for (int j = tid; j < old; j += ET) {
+                    const unsigned k = key(j);
+                    if (k >> (shift + width) == high) atomicAdd(&s.bins[k >> shift & mask], 1u);
+                }
             }
             __syncthreads();
             // from the largest digit down: four a thread
@@ -138,7 +168,11 @@ __global__ void __launch_bounds__(ET, 2) kv4_evict_kernel(Kv4 src, Kv4 dst, cons
             for (int w = 0; w < warp; ++w) before += s.warp_n[w];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                if (before < ties && before + n[i] >= ties) { s.digit = BINS - 1 - (4 * tid + i); s.above = before; }
+                if (before < ties && before + n[i] >= ties) {
+                    s.digit = BINS - 1 - (4 * tid + i);
+                    s.above = before;
+                    if (pass == 0) s.in_bin = n[i];
+                }
                 before += n[i];
             }
             __syncthreads();
@@ -189,11 +223,13 @@ __global__ void __launch_bounds__(ET, 2) kv4_evict_kernel(Kv4 src, Kv4 dst, cons
         const int body = all ? 0 : want;
         for (int to = max(w0, body) + tid; to < w1; to += ET) s.src[to - w0] = all ? to : to - body + old;
         __syncthreads();
+#pragma unroll 4
         for (int e = tid; e < rows * nb; e += ET) {
             const int i = e / nb, q = e % nb;
             ((uint4*)(dst.kq + (da + w0 + i) * (nb * 4)))[q] = __ldg((const uint4*)(src.kq + (sa + s.src[i]) * (nb * 4)) + q);
         }
         const int pairs = rows >> 1;
+#pragma unroll 4
         for (int e = tid; e < pairs * 2 * nb; e += ET) {
             const int i = e / (2 * nb), q = e % (2 * nb), a = s.src[2 * i], b = s.src[2 * i + 1];
             const uint4 x = __ldg((const uint4*)(src.vq + ((sa + a) >> 1) * (nb * 8)) + q), y = __ldg((const uint4*)(src.vq + ((sa + b) >> 1) * (nb * 8)) + q);
@@ -207,10 +243,12 @@ __global__ void __launch_bounds__(ET, 2) kv4_evict_kernel(Kv4 src, Kv4 dst, cons
             uint16_t* y = (uint16_t*)(dst.vq + ((da + w1 - 1) / 2) * (nb * 8));
             for (int e = tid; e < 8 * nb; e += ET) y[2 * e] = x[2 * e];
         }
+#pragma unroll 4
         for (int e = tid; e < rows * nb; e += ET) {
             const int i = e / nb, q = e % nb;
-            dst.kd[(da + w0) * nb + e] = src.kd[(sa + s.src[i]) * nb + q];
-            dst.vd[(da + w0) * nb + e] = src.vd[(sa + s.src[i]) * nb + q];
+            const uint16_t k = __ldg((const uint16_t*)src.kd + (sa + s.src[i]) * nb + q), v = __ldg((const uint16_t*)src.vd + (sa + s.src[i]) * nb + q);
+            ((uint16_t*)dst.kd)[(da + w0) * nb + e] = k;
+            ((uint16_t*)dst.vd)[(da + w0) * nb + e] = v;
         }
         for (int i = tid; i < rows; i += ET) {
             if (mass_out) mass_out[(size_t)head * dst.cap + w0 + i] = m[s.src[i]];
@@ -340,8 +378,8 @@ int fc_kv4_read_dev(const fc_kv4* c, const int32_t* from, int n, float* k, float
     if (!n) return FC_OK;
     FC_TRY(make_device(c->device));
     if (!aligned16(k) || !aligned16(v)) return fail(FC_E_ARG, "fc_kv4_read_dev: k and v must be 16-byte aligned");
-    const size_t all = (size_t)n * c->c.n_kv * c->c.nb * 8;
-    const dim3 grid((unsigned)std::min<size_t>((all + 255) / 256, 148 * 16), c->c.n_seq);
+    const int per = 128 / (c->c.nb * 4);
+    const dim3 grid((unsigned)std::min<long long>(((long long)n * c->c.n_kv + per - 1) / per, std::max(1, 148 * 16 / c->c.n_seq)), c->c.n_seq);
     kv4_read_kernel<<<grid, 256, 0, (cudaStream_t)stream>>>(c->c, from, n, k, v);
     FC_LAUNCHED();
     return FC_OK;

@@ -5,12 +5,14 @@
 //
 // Weights are exp((l - max) / T), computed in f64 and summed as whole numbers of 2^-42: a flat row of 2^17 ids has borders 2^-17 apart, of
 // which sums in 32 bits miss one in a hundred; whole numbers can be added in any order. The exponential is Tang's (Table-driven
-// implementation of the exponential function, ACM TOMS 15, 1989): 2^(i / 16) from a table that fills the 32 banks once, times a
-// polynomial of degree 5.
+// implementation of the exponential function, ACM TOMS 15, 1989): 2^(i / 64) from a table, times a polynomial of degree 3, to 4e-11.
 //
-// A cluster of CTAs shares a row and reads it up to four times, from L2 after the first: (1) the largest and the least; (2) the weights,
-// their sums by chunk and, if there is a top-k or top-p, by value in 1024 buckets; (3) if there is, the bucket in which the cut lies is
-// listed and searched; then the chunks' sums of what stays. The chunk that the random number falls into is walked by one warp.
+// A cluster of CTAs shares a row and passes over it two or three times: (1) the largest and the least; (2) for a top-k or top-p, counts
+// and f32 masses by value in 2048 buckets, which say in which few of them the cut lies; (3) the exact weights, summed
+// by chunk above those buckets, listed in them. The list gives the cut, exactly; if it does not hold the cut after all, or not all of
+// them, bisection finds it. The chunk that the random number falls into is walked by one warp.
+//
+// Bound: the instructions of the passes (a weight is 9 operations in f64 and some thirty in all), and for few rows their latency.
 #include <cooperative_groups.h>
 
 #include "fc_common.cuh"
@@ -21,63 +23,66 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int RT = 512, RW = RT / 32, BUCKETS = 1024, LIST = 1024, CHUNKS = 512;
+constexpr int RT = 256, RW = RT / 32, BUCKETS = 2048, PER = BUCKETS / RT, LIST = 1024, CHUNKS = 512;
 constexpr int kFix = 42;                      // weights are whole numbers of 2^-42; rows of up to 2^20 of them stay below 2^63
 constexpr int kMaxVocab = 1 << 20;
+constexpr int kPairs = 160;                   // entries of a list that are compared each with each (at most a thread each)
+constexpr int kSlice = 40960;                 // ids of a CTA that shared memory holds
 constexpr double kLeast = -40.0;              // weights under 2^-40 are not drawn
 using u64 = unsigned long long;
 
-// Logits in their order as unsigned keys.
+// Logits in their order as unsigned keys, and back.
 __device__ __forceinline__ unsigned logit_key(float l) {
     const unsigned b = __float_as_uint(l + 0.0f);
     return b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u);
 }
+__device__ __forceinline__ float key_logit(unsigned k) { return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k); }
 
 struct Row {
     const float* p;
     int V;
-    bool vec, endless;                        // 16-byte aligned; the largest is infinite
-    // NaN is a forbidden id, as -inf; among infinities the others weigh nothing
-    __device__ __forceinline__ float fix(float l) const {
-        l = l == l ? l : -INFINITY;
-        return endless ? (l == INFINITY ? 0.0f : -INFINITY) : l;
-    }
-    __device__ __forceinline__ void load4(int i, float (&v)[4]) const {
-        if (vec && i + 3 < V) {
-            const float4 x = __ldg((const float4*)(p + i));
-            v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
-        } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = i + e < V ? __ldg(p + i + e) : -INFINITY;
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = fix(v[e]);
+    bool vec;                                 // 16-byte aligned
+    // NaN is a forbidden id, as -inf
+    static __device__ __forceinline__ float fix(float l) { return fmaxf(l, -INFINITY); }
+    // four ids from i on as they are: a load in flight has no reader yet
+    __device__ __forceinline__ float4 load4(int i) const {
+        if (vec && i + 3 < V) return __ldg((const float4*)(p + i));
+        float4 v;
+        v.x = i < V ? __ldg(p + i) : -INFINITY;
+        v.y = i + 1 < V ? __ldg(p + i + 1) : -INFINITY;
+        v.z = i + 2 < V ? __ldg(p + i + 2) : -INFINITY;
+        v.w = i + 3 < V ? __ldg(p + i + 3) : -INFINITY;
+        return v;
     }
 };
 
 struct Weigher {
-    double best, scale;                       // log2(e) / T
-    float least;                              // logits below it weigh nothing: 2^-45 at most
+    double scale, shift;                      // log2(e) / T; what brings the largest to 0
+    float least;                              // logits below it weigh nothing (2^-45 at most): they are not asked for
+    float top;                                // asked for in the place of what does not count
     const double* table;
-    __device__ __forceinline__ double log2w(float l) const { return ((double)l - best) * scale; }
-    // 2^(x + up) for -1000 <= x <= 0: x = (16 n + i) / 16 + r, |r| <= 1 / 32
-    __device__ __forceinline__ double power(double x, int up) const {
-        const double magic = 6755399441055744.0 / 16.0;      // 1.5 * 2^52 / 16: the sum's last bits are 16 x, rounded
+    __device__ __forceinline__ double log2w(float l) const { return fma((double)l, scale, shift); }
+    // 2^(x + up) - z, z its table entry with the exponent, for -1000 <= x <= 0: x = (64 n + i) / 64 + r, |r| <= 1 / 128
+    __device__ __forceinline__ double power(double x, int up, double* z) const {
+        const double magic = 6755399441055744.0 / 64.0;      // 1.5 * 2^52 / 64: the sum's last bits are 64 x, rounded
         const double t = x + magic;
         const int k = __double2loint(t);
-        const double r = x - (t - magic);
-        double y = fma(r, 1.3333558146428443e-3, 9.6181291076284772e-3);
-        y = fma(r, y, 5.5504108664821580e-2);
-        y = fma(r, y, 2.4022650695910071e-1);
-        y = fma(r, y, 6.9314718055994531e-1);
-        y = fma(r, y, 1.0) * table[k & 15];                  // in [0.97, 2)
-        return __hiloint2double(__double2hiint(y) + ((k >> 4) + up) * (1 << 20), __double2loint(y));
+        const double r = x - (t - magic), e = table[k & 63];
+        *z = __hiloint2double(__double2hiint(e) + ((k >> 6) + up) * (1 << 20), __double2loint(e));
+        return r * fma(r, fma(r, 5.5504108664821580e-2, 2.4022650695910071e-1), 6.9314718055994531e-1);
     }
-    // the sum's last bits are the weight in units of 2^-42, rounded
-    __device__ __forceinline__ u64 fixed(double x) const {
-        return (u64)__double_as_longlong(power(x, kFix) + 4503599627370496.0) & 0xfffffffffffffull;
+    // the sum's last bits are the weight in units of 2^-42, rounded; 0 for what does not count
+    __device__ __forceinline__ u64 fixed(float l, bool counts = true) const {
+        double z;
+        const double q = power(log2w(counts ? l : top), kFix, &z);
+        z = __hiloint2double(counts ? __double2hiint(z) : 0, __double2loint(z));
+        return (u64)__double_as_longlong(fma(z, q, z + 4503599627370496.0)) & 0xfffffffffffffull;
     }
-    __device__ __forceinline__ double exact(double x) const { return power(x, 0); }
+    __device__ __forceinline__ double exact(float l) const {
+        double z;
+        const double q = power(log2w(l), 0, &z);
+        return fma(z, q, z);
+    }
 };
 
 __device__ __forceinline__ u64 warp_sum(u64 v) {
@@ -86,75 +91,136 @@ __device__ __forceinline__ u64 warp_sum(u64 v) {
     return v;
 }
 
-struct Shared {
-    unsigned cnt[BUCKETS], lo[BUCKETS], hi[BUCKETS];      // this CTA's buckets
-    unsigned all_cnt[BUCKETS];                            // the cluster's
-    u64 all_mass[BUCKETS];
+struct __align__(16) Shared {
+    unsigned cnt[BUCKETS], mass[BUCKETS];                 // this CTA's buckets
+    union {
+        struct {                                          // the cluster's, until the cut's buckets are known
+            unsigned all_cnt[BUCKETS];
+            float all_mass[BUCKETS];
+        };
+        struct {                                          // what lies in them
+            u64 list_w[LIST];
+            unsigned list_key[LIST];
+            unsigned short list_chunk[LIST];
+        };
+    };
     u64 chunk[CHUNKS];
-    u64 list_w[LIST];
-    unsigned list_key[LIST];
-    double table[16];
-    u64 warp_w[RW], whole, sum, sums[16];
+    double table[64];
+    u64 warp_w[RW], above_w, list_all, whole, sum;
+    float warp_f[RW];
     unsigned warp_n[RW];
-    float most, least, tops[16], lows[16];
-    int first, firsts[16];
-    int listed, bucket;
-    u64 above_w;
-    unsigned above_n, cut;
-    int wants;                                            // 1: top-k cuts in the bucket, 2: top-p does
-    u64 wide_w;                                           // sums of a pass of the fallback
+    float most, least, tops[RW], lows[RW];
+    int first, firsts[RW];
+    int listed, b1, b2;
+    unsigned above_n, cut, found;
+    unsigned pair_n[2][RW];
+    u64 pair_w[2][RW];
+    u64 wide_w;                                           // sums of a pass of the bisection
     unsigned wide_n;
 };
 
-// A pass over the CTA's chunks: f(values, index of the first, chunk) for four ids a lane.
-template <class F>
-__device__ __forceinline__ void over(const Row& row, int begin, int end, int chunk, const F& f) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    for (int c = warp, i0 = begin + warp * chunk; i0 < end; c += RW, i0 += RW * chunk) {
-        const int stop = min(i0 + chunk, end);
-        for (int i = i0 + 4 * lane; i - 4 * lane < stop; i += 128) {
-            float v[4];
-            if (i < stop) row.load4(i, v);
-            else v[0] = v[1] = v[2] = v[3] = -INFINITY;
-            f(v, i, c);
-        }
-        f.done(c);
-    }
-}
+static_assert(sizeof(Shared) % 16 == 0, "the slice behind it is read in 16-byte words");
 
-__global__ void __launch_bounds__(RT, 2) sample_rows_kernel(const float* __restrict__ logits, long long ld, int V, const fc_row_sampling* __restrict__ params,
-                                                            const float* __restrict__ u, int* __restrict__ token, float* __restrict__ prob, int cs, int chunk) {
+// The ids that a CTA holds, in chunks that the warps take in turn: in shared memory (slice) behind the first pass where they fit.
+struct Share {
+    Row row;
+    int begin, end, chunk;
+    float* slice;
+    bool endless;                             // the largest is infinite: among infinities the others weigh nothing
+    __device__ __forceinline__ float settle(float l) const { return endless ? (l == INFINITY ? 0.0f : -INFINITY) : l; }
+    __device__ __forceinline__ float at(int i) const { return settle(slice ? slice[i - begin] : Row::fix(__ldg(row.p + i))); }
+    // f(values, chunk) for four ids a lane, f.done(chunk) behind each chunk; up to four loads of a lane are on their way
+    template <class F>
+    __device__ __forceinline__ void over(const F& f) const {
+        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, steps = chunk / 128;
+        auto give = [&](const float4& x, int c) {
+            float v[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = Row::fix(v[e]);
+            if (endless) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = settle(v[e]);
+            }
+            f(v, c);
+        };
+        const float4 none = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+        if (slice) {
+            for (int c = warp, i0 = begin + warp * chunk; i0 < end; c += RW, i0 += RW * chunk) {
+                for (int q = 0; q < steps; ++q)
+                    if (i0 + 128 * q < end) give(*(const float4*)(slice + i0 - begin + 128 * q + 4 * lane), c);
+                f.done(c);
+            }
+            return;
+        }
+        // the warp's pieces of 128 ids in order: piece j is step j % steps (a power of two) of its chunk j / steps
+        const int bits = 31 - __clz(steps);
+        const int chunks = end > begin + warp * chunk ? (end - begin - warp * chunk + RW * chunk - 1) / (RW * chunk) : 0, pieces = chunks * steps;
+        auto place = [&](int j) { return begin + (warp + (j >> bits) * RW) * chunk + (j & (steps - 1)) * 128 + 4 * lane; };
+        for (int j0 = 0; j0 < pieces; j0 += 4) {
+            float4 x[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int i = place(j0 + q);
+                x[q] = j0 + q < pieces && i < end ? row.load4(i) : none;
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int j = j0 + q;
+                if (j >= pieces) break;
+                const int c = warp + (j >> bits) * RW;
+                give(x[q], c);
+                if (((j + 1) & (steps - 1)) == 0) f.done(c);
+            }
+        }
+    }
+};
+
+__global__ void __launch_bounds__(RT, 4) sample_rows_kernel(const float* __restrict__ logits, long long ld, int V, const fc_row_sampling* __restrict__ params,
+                                                            const float* __restrict__ u, int* __restrict__ token, float* __restrict__ prob, int cs, int chunk, int in_shared) {
     extern __shared__ __align__(16) char smem_raw[];
     Shared& s = *(Shared*)smem_raw;
     cg::cluster_group cluster = cg::this_cluster();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, rank = blockIdx.x % cs, r = blockIdx.x / cs;
     const fc_row_sampling p = params[r];
-    Row row = {logits + (size_t)r * ld, V, false, false};
-    row.vec = ((uintptr_t)row.p & 15) == 0;
+    const float* const in = logits + (size_t)r * ld;
     // whole chunks a CTA
     const int share = ((V + cs - 1) / cs + chunk - 1) / chunk * chunk, begin = min(V, rank * share), end = min(V, begin + share);
+    Share ids = {{in, V, ((uintptr_t)in & 15) == 0}, begin, end, chunk, in_shared ? (float*)(smem_raw + sizeof(Shared)) : nullptr, false};
     auto sync = [&]() { if (cs > 1) cluster.sync(); else __syncthreads(); };
     auto at = [&](auto* x, int q) { return cs > 1 ? cluster.map_shared_rank(x, q) : x; };
 
-    // 1. the largest, where it comes first, and the least finite one
-    struct Extremes {
-        float &top, &low;
-        int& first;
-        __device__ void operator()(const float (&v)[4], int i, int) const {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                if (v[e] > top) { top = v[e]; first = i + e; }
-                if (v[e] > -INFINITY) low = fminf(low, v[e]);
-            }
-        }
-        __device__ void done(int) const {}
-    };
+    // 1. the largest, where it comes first, and the least finite one; four loads of a lane on their way at a time
     float top = -INFINITY, low = INFINITY;
     int first = V;
-    over(row, begin, end, chunk, Extremes{top, low, first});
-    if (tid < 16) s.table[tid] = exp2((double)tid * 0.0625);
-    for (int b = tid; b < BUCKETS; b += RT) s.cnt[b] = s.lo[b] = s.hi[b] = 0;
-    if (tid < CHUNKS) s.chunk[tid] = 0;
+    for (int i0 = begin; i0 < end; i0 += 16 * RT) {
+        float4 x[4];
+        if (ids.row.vec && i0 + 16 * RT <= end) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) x[q] = __ldg((const float4*)(in + i0 + 4 * (q * RT + tid)));
+        } else {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) x[q] = ids.row.load4(i0 + 4 * (q * RT + tid));
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int i = i0 + 4 * (q * RT + tid);
+            if (i >= end) continue;
+            const float v[4] = {Row::fix(x[q].x), Row::fix(x[q].y), Row::fix(x[q].z), Row::fix(x[q].w)};
+            if (ids.slice) *(float4*)(ids.slice + i - begin) = make_float4(v[0], v[1], v[2], v[3]);
+            const float most = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]));
+            if (most > top) {
+                top = most;
+                first = i + (v[0] == most ? 0 : v[1] == most ? 1 : v[2] == most ? 2 : 3);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) low = fminf(low, v[e] > -INFINITY ? v[e] : INFINITY);
+        }
+    }
+    // what a chunk's last quarters read behind the end
+    if (ids.slice)
+        for (int i = ((end - begin + 3) & ~3) + tid; i < share; i += RT) ids.slice[i] = -INFINITY;
+    if (tid < 64) s.table[tid] = exp2((double)tid * 0.015625);
+    for (int b = tid; b < BUCKETS; b += RT) s.cnt[b] = s.mass[b] = 0;
     auto better = [](float a, int i, float b, int j) { return a > b || (a == b && i < j); };
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
@@ -171,7 +237,7 @@ __global__ void __launch_bounds__(RT, 2) sample_rows_kernel(const float* __restr
             low = fminf(low, s.lows[w]);
         }
         s.most = top; s.least = low; s.first = first;
-        s.listed = 0;
+        s.listed = 0; s.b1 = s.b2 = BUCKETS; s.found = 0;
     }
     sync();
     top = -INFINITY; low = INFINITY; first = V;
@@ -187,236 +253,314 @@ __global__ void __launch_bounds__(RT, 2) sample_rows_kernel(const float* __restr
         if (cs > 1) cluster.sync();           // no rank leaves while another reads its memory
         return;
     }
-    row.endless = top == INFINITY;
-    if (row.endless) { top = low = 0.0f; }
+    ids.endless = top == INFINITY;
+    if (ids.endless) { top = low = 0.0f; }
 
-    const double temp = fmax((double)p.temperature, 0.01);
+    const double temp = fmin(fmax((double)p.temperature, 0.01), 1e30);
     // (45 / log2(e) = 31.2; a rounding of the product or the difference does not reach 2^-43)
-    const Weigher weigh = {(double)top, 1.4426950408889634 / temp, top - 31.25f * (float)fmin(temp, 1e30), s.table};
+    const double scale = 1.4426950408889634 / temp;
+    const Weigher weigh = {scale, -(double)top * scale, top - 31.25f * (float)temp, top, s.table};
     const bool cut_k = p.top_k > 0 && p.top_k < V, cut_p = p.top_p < 1.0f;
+    // the least logit that min-p, and 2^-40, let stay: the weight falls with the logit, so that one comparison in f32 decides
     const double floor_x = p.min_p > 0.0f ? fmax(log2(fmin((double)p.min_p, 1.0)), kLeast) : kLeast;
-    // buckets of even width from the largest down to what has a weight
-    const float range = fminf(top - low, 30.5f * (float)fmin(temp, 1e30)), per = range > 0.0f ? (float)(BUCKETS - 1) / range : 0.0f;
-    auto bucket_of = [&](float l) { return min((int)fminf((top - l) * per, (float)(BUCKETS - 1)), BUCKETS - 1); };
+    float keep = (float)fmax((double)top + floor_x / scale, -3.4e38);
+    for (int i = 0; i < 4 && keep > -3.4e38f && weigh.log2w(keep) >= floor_x; ++i) keep = nextafterf(keep, -INFINITY);
+    for (int i = 0; i < 8 && keep < top && weigh.log2w(keep) < floor_x; ++i) keep = nextafterf(keep, INFINITY);
 
-    // 2. the weights: of the whole row where a cut has to be found, else of what stays
-    struct Weigh {
+    u64 lane_sum = 0, warp_all = 0, lane_all = 0;
+    // the weights of what is not below `keep`, by chunk; a chunk's lanes without any skip them
+    struct Keep {
         Shared& s;
         const Weigher& weigh;
-        const decltype(bucket_of)& bucket;
-        double floor_x;
-        bool by_value, count_too, mass_too;
+        float keep;
         int lane;
         u64& sum;
         u64& all;
-        __device__ void operator()(const float (&v)[4], int, int) const {
+        __device__ __forceinline__ void operator()(const float (&v)[4], int) const {
+            if (!__any_sync(0xffffffffu, fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])) >= keep)) return;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                if (v[e] == -INFINITY) continue;
-                const bool weighs = v[e] >= weigh.least;
-                if (by_value) {
-                    const u64 w = mass_too && weighs ? weigh.fixed(weigh.log2w(v[e])) : 0;
-                    const int b = bucket(v[e]);
-                    if (count_too) atomicAdd(&s.cnt[b], 1u);
-                    if (w) {
-                        const unsigned lo = (unsigned)w, old = atomicAdd(&s.lo[b], lo);
-                        const unsigned hi = (unsigned)(w >> 32) + (old + lo < lo);
-                        if (hi) atomicAdd(&s.hi[b], hi);
-                    }
-                } else if (weighs) {
-                    const double x = weigh.log2w(v[e]);
-                    if (x >= floor_x) sum += weigh.fixed(x);
-                }
-            }
+            for (int e = 0; e < 4; ++e) sum += weigh.fixed(v[e], v[e] >= keep);
         }
-        __device__ void done(int c) const {
-            if (by_value) return;
+        __device__ __forceinline__ void done(int c) const {
             const u64 w = warp_sum(sum);
             all += w;
             sum = 0;
             if (lane == 0) s.chunk[c] = w;
         }
     };
-    u64 lane_sum = 0, warp_all = 0;
-    const bool by_value = cut_k || cut_p;
-    over(row, begin, end, chunk, Weigh{s, weigh, bucket_of, floor_x, by_value, cut_k, cut_p, lane, lane_sum, warp_all});
-    unsigned cut = 0;
-    if (by_value) {
-        sync();
-        // each rank adds up its share of the buckets and hands it to all
-        const int per_rank = BUCKETS / cs;
-        for (int b = rank * per_rank + tid; b < (rank + 1) * per_rank; b += RT) {
-            unsigned n = 0;
-            u64 w = 0;
-            for (int q = 0; q < cs; ++q) {
-                n += *at(&s.cnt[b], q);
-                w += (u64)*at(&s.hi[b], q) << 32;
-                w += *at(&s.lo[b], q);
-            }
-            for (int q = 0; q < cs; ++q) { *at(&s.all_cnt[b], q) = n; *at(&s.all_mass[b], q) = w; }
-        }
-        sync();
-        // two buckets a thread: what lies above them
-        static_assert(BUCKETS == 2 * RT, "two buckets a thread");
-        const unsigned n0 = s.all_cnt[2 * tid], n1 = s.all_cnt[2 * tid + 1];
-        const u64 w0 = s.all_mass[2 * tid], w1 = s.all_mass[2 * tid + 1];
-        unsigned n = n0 + n1;
-        u64 w = w0 + w1;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const unsigned n2 = __shfl_up_sync(0xffffffffu, n, o);
-            const u64 w2 = __shfl_up_sync(0xffffffffu, w, o);
-            if (lane >= o) { n += n2; w += w2; }
-        }
-        if (lane == 31) { s.warp_n[warp] = n; s.warp_w[warp] = w; }
-        if (tid == 0) { s.bucket = BUCKETS; s.wants = 0; }
-        __syncthreads();
-        u64 whole = 0;
-        for (int q = 0; q < RW; ++q) {
-            if (q < warp) { n += s.warp_n[q]; w += s.warp_w[q]; }
-            whole += s.warp_w[q];
-        }
-        const double want = (double)p.top_p * (double)whole;
-        auto reached = [&](u64 m) { return (double)m >= want; };
-        // the first bucket (from the largest down) at whose end k ids, or the mass, are there
-        unsigned an = n - n0 - n1;
-        u64 aw = w - w0 - w1;
-        int mine = BUCKETS;
-#pragma unroll
-        for (int i = 1; i >= 0; --i) {
-            const unsigned bn = i ? n : n - n1;
-            const u64 bw = i ? w : w - w1;
-            const bool k = cut_k && bn >= (unsigned)p.top_k, m = cut_p && reached(bw);
-            if (k || m) mine = 2 * tid + i;
-        }
-        if (mine < BUCKETS) atomicMin(&s.bucket, mine);
-        __syncthreads();
-        if (mine == s.bucket) {
-            const int i = mine & 1;
-            s.above_n = i ? an + n0 : an;
-            s.above_w = i ? aw + w0 : aw;
-            s.wants = (cut_k && (i ? n : n - n1) >= (unsigned)p.top_k ? 1 : 0) | (cut_p && reached(i ? w : w - w1) ? 2 : 0);
-        }
-        __syncthreads();
-        const int bucket = s.bucket, wants = s.wants;
-        if (bucket < BUCKETS) {
-            // 3. the cut: the largest value of this bucket down to which k ids, or the mass, are there
-            const unsigned above_n = s.above_n;
-            const u64 above_w = s.above_w;
-            auto enough = [&](unsigned k, u64 m) { return ((wants & 1) && above_n + k >= (unsigned)p.top_k) || ((wants & 2) && reached(above_w + m)); };
-            bool listed = !cut_k || s.all_cnt[bucket] <= LIST;
-            if (listed) {
-                struct Gather {
-                    Shared& s;
-                    const Weigher& weigh;
-                    const decltype(bucket_of)& bucket;
-                    int* listed;
-                    unsigned* keys;
-                    u64* ws;
-                    int which;
-                    __device__ void operator()(const float (&v)[4], int, int) const {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (v[e] > -INFINITY && bucket(v[e]) == which) {
-                                const int q = atomicAdd(listed, 1);
-                                if (q >= LIST) continue;
-                                keys[q] = logit_key(v[e]);
-                                ws[q] = v[e] >= weigh.least ? weigh.fixed(weigh.log2w(v[e])) : 0;
-                            }
-                    }
-                    __device__ void done(int) const {}
-                };
-                over(row, begin, end, chunk, Gather{s, weigh, bucket_of, at(&s.listed, 0), at(s.list_key, 0), at(s.list_w, 0), bucket});
-                sync();
-                listed = *at(&s.listed, 0) <= LIST;
-                if (rank == 0 && listed) {
-                    const int n = s.listed;
-                    for (int i = tid; i < n; i += RT) {
-                        const unsigned key = s.list_key[i];
-                        unsigned ge = 0, gt = 0;
-                        u64 wge = 0, wgt = 0;
-                        for (int q = 0; q < n; ++q) {
-                            const unsigned k = s.list_key[q];
-                            const u64 x = s.list_w[q];
-                            if (k >= key) { ++ge; wge += x; }
-                            if (k > key) { ++gt; wgt += x; }
-                        }
-                        // all of a tie write the same
-                        if (enough(ge, wge) && !(gt && enough(gt, wgt))) for (int q = 0; q < cs; ++q) *at(&s.cut, q) = key;
-                    }
-                }
-                sync();
-                cut = listed ? s.cut : 0;
-            }
-            if (!listed) {
-                // more of them than the list holds: the cut's bits from the highest down, a pass each
-                struct Count {
-                    Shared& s;
-                    const Weigher& weigh;
-                    const decltype(bucket_of)& bucket;
-                    int which;
-                    unsigned cand;
-                    unsigned& n;
-                    u64& w;
-                    bool mass_too;
-                    __device__ void operator()(const float (&v)[4], int, int) const {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (v[e] > -INFINITY && logit_key(v[e]) >= cand && bucket(v[e]) == which) {
-                                ++n;
-                                if (mass_too && v[e] >= weigh.least) w += weigh.fixed(weigh.log2w(v[e]));
-                            }
-                    }
-                    __device__ void done(int) const {}
-                };
-                for (int bit = 31; bit >= 0; --bit) {
-                    const unsigned cand = cut | (1u << bit);
-                    unsigned n = 0;
-                    u64 w = 0;
-                    over(row, begin, end, chunk, Count{s, weigh, bucket_of, bucket, cand, n, w, (wants & 2) != 0});
-                    n = __reduce_add_sync(0xffffffffu, n);
-                    w = warp_sum(w);
-                    if (lane == 0) { s.warp_n[warp] = n; s.warp_w[warp] = w; }
-                    __syncthreads();
-                    if (tid == 0) {
-                        for (int q = 1; q < RW; ++q) { n += s.warp_n[q]; w += s.warp_w[q]; }
-                        s.wide_n = n; s.wide_w = w;
-                    }
-                    sync();
-                    n = 0; w = 0;
-                    for (int q = 0; q < cs; ++q) { n += *at(&s.wide_n, q); w += *at(&s.wide_w, q); }
-                    if (n && enough(n, w)) cut = cand;
-                    sync();
-                }
-            }
-        }
-        // the chunks' sums of what stays
-        struct Keep {
+    if (!cut_k && !cut_p) {
+        ids.over(Keep{s, weigh, keep, lane, lane_sum, warp_all});
+    } else {
+        // 2. buckets of even width from the largest down to what has a weight. A bucket's mass is in units of a
+        // part of its middle's weight, as small as all ids in one bucket allow.
+        const float range = fminf(top - low, 31.25f * (float)temp), per = range > 0.0f ? (float)(BUCKETS - 1) / range : 0.0f;
+        const float unit = (float)(1u << min(30 - (32 - __clz(V)), 22)), slope = (float)weigh.scale, width = range > 0.0f ? range / (float)(BUCKETS - 1) * slope : 0.0f;      // in powers of two
+        // (2^23 + n has n in its low bits)
+        auto bucket_of = [&](float l) { return __float_as_int(fminf((top - l) * per, (float)(BUCKETS - 1)) + 8388608.0f) & (2 * BUCKETS - 1); };
+        struct Sort {
             Shared& s;
-            const Weigher& weigh;
-            double floor_x;
-            unsigned cut;
-            int lane;
-            u64& sum;
-            u64& all;
-            __device__ void operator()(const float (&v)[4], int, int) const {
+            const decltype(bucket_of)& bucket;
+            float top, slope, width, unit;
+            bool count_too, mass_too;
+            __device__ __forceinline__ void operator()(const float (&v)[4], int) const {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    if (!(v[e] >= weigh.least) || logit_key(v[e]) < cut) continue;
-                    const double x = weigh.log2w(v[e]);
-                    if (x >= floor_x) sum += weigh.fixed(x);
+                    const int b = bucket(v[e]);
+                    if (count_too && v[e] > -INFINITY) atomicAdd(&s.cnt[b], 1u);
+                    if (mass_too) {
+                        // (in the last bucket, what lies behind the range comes to nothing)
+                        const float x = fmaf(v[e] - top, slope, (float)b * width);
+                        float w;
+                        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w) : "f"(x));
+                        const unsigned m = (unsigned)__float_as_int(fmaf(w, unit, 8388608.0f)) - 0x4b000000u;
+                        if (m) atomicAdd(&s.mass[b], m);
+                    }
                 }
             }
-            __device__ void done(int c) const {
+            __device__ __forceinline__ void done(int) const {}
+        };
+        ids.over(Sort{s, bucket_of, top, slope, width, unit, cut_k, cut_p});
+        sync();
+        // each rank adds up its share of the buckets and hands it to all
+        for (int b = rank * RT + tid; b < BUCKETS; b += cs * RT) {
+            unsigned n = 0;
+            u64 m = 0;
+            for (int q = 0; q < cs; ++q) {
+                n += *at(&s.cnt[b], q);
+                m += *at(&s.mass[b], q);
+            }
+            const float mass = (float)m * exp2f(-(float)b * width);
+            for (int q = 0; q < cs; ++q) { *at(&s.all_cnt[b], q) = n; *at(&s.all_mass[b], q) = mass; }
+        }
+        sync();
+        // PER buckets a thread: how many ids and how much mass there are at the end of each
+        unsigned bn[PER], n = 0;
+        float bm[PER], m = 0.0f;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            n += s.all_cnt[PER * tid + i]; bn[i] = n;
+            m += s.all_mass[PER * tid + i]; bm[i] = m;
+        }
+        unsigned an = n;
+        float am = m;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const unsigned n2 = __shfl_up_sync(0xffffffffu, an, o);
+            const float m2 = __shfl_up_sync(0xffffffffu, am, o);
+            if (lane >= o) { an += n2; am += m2; }
+        }
+        if (lane == 31) { s.warp_n[warp] = an; s.warp_f[warp] = am; }
+        __syncthreads();
+        float all_m = 0.0f;
+        for (int q = 0; q < RW; ++q) {
+            if (q < warp) { an += s.warp_n[q]; am += s.warp_f[q]; }
+            all_m += s.warp_f[q];
+        }
+        an -= n; am -= m;
+        // the cut lies behind b1 - 1 and not behind b2: ids are counted, the mass is sure to half a unit of weights of 0.98 units and above, and
+        // to the roundings in f32 of a logarithm below 2^6
+        const float want_m = p.top_p * all_m, slack = all_m * (0.6f / unit + 1.5e-5f);
+        int b1 = BUCKETS, b2 = BUCKETS;
+#pragma unroll
+        for (int i = PER - 1; i >= 0; --i) {
+            const bool k = cut_k && an + bn[i] >= (unsigned)p.top_k;
+            if (k || (cut_p && am + bm[i] >= want_m - slack)) b1 = PER * tid + i;
+            if (k || (cut_p && am + bm[i] >= want_m + slack)) b2 = PER * tid + i;
+        }
+        if (b1 < BUCKETS) atomicMin(&s.b1, b1);
+        if (b2 < BUCKETS) atomicMin(&s.b2, b2);
+        __syncthreads();
+        b1 = s.b1; b2 = min(s.b2, BUCKETS - 1);
+        sync();                               // the list lies where the buckets were
+        if (b1 - 1 >= PER * tid && b1 - 1 < PER * (tid + 1)) s.above_n = an + bn[(b1 - 1) % PER];
+        if (b1 == 0 && tid == 0) s.above_n = 0;
+
+        // 3. the weights: above those buckets by chunk, in them listed, below them only for the whole
+        struct List {
+            Shared& s;
+            const Weigher& weigh;
+            const decltype(bucket_of)& bucket;
+            float keep;
+            int b1, b2, lane;
+            bool whole;
+            u64& sum;
+            u64& all;
+            u64& above;
+            __device__ __forceinline__ void operator()(const float (&v)[4], int c) const {
+                const float most = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]));
+                if (!__any_sync(0xffffffffu, (whole ? most >= weigh.least : most > -INFINITY && bucket(most) <= b2))) return;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const u64 w = weigh.fixed(v[e], v[e] >= weigh.least);
+                    const int b = bucket(v[e]);
+                    all += w;
+                    above += b < b1 ? w : 0;
+                    sum += b < b1 && v[e] >= keep ? w : 0;
+                    if (b >= b1 && b <= b2 && v[e] > -INFINITY) {
+                        const int q = atomicAdd(&s.listed, 1);
+                        if (q < LIST) { s.list_key[q] = logit_key(v[e]); s.list_w[q] = w; s.list_chunk[q] = (unsigned short)c; }
+                    }
+                }
+            }
+            __device__ __forceinline__ void done(int c) const {
                 const u64 w = warp_sum(sum);
-                all += w;
                 sum = 0;
                 if (lane == 0) s.chunk[c] = w;
             }
         };
-        over(row, begin, end, chunk, Keep{s, weigh, floor_x, cut, lane, lane_sum, warp_all});
+        u64 lane_above = 0;
+        ids.over(List{s, weigh, bucket_of, keep, b1, b2, lane, cut_p, lane_sum, lane_all, lane_above});
+        lane_all = warp_sum(lane_all);
+        lane_above = warp_sum(lane_above);
+        __syncthreads();                      // the warps' sums of the buckets have been read
+        if (lane == 0) { s.warp_w[warp] = lane_all; s.list_all = 0; s.above_w = 0; }
+        __syncthreads();
+        if (lane == 0) atomicAdd(&s.above_w, lane_above);
+        if (tid == 0) {
+            u64 w = 0;
+            for (int q = 0; q < RW; ++q) w += s.warp_w[q];
+            s.whole = w;
+        }
+        sync();
+        u64 whole = 0, above_w = 0;
+        int total = 0;
+        for (int q = 0; q < cs; ++q) { whole += *at(&s.whole, q); above_w += *at(&s.above_w, q); total += *at(&s.listed, q); }
+        const unsigned above_n = s.above_n;
+        const double want = (double)p.top_p * (double)whole;
+        auto enough = [&](unsigned k, u64 w) { return (cut_k && k >= (unsigned)p.top_k) || (cut_p && (double)w >= want); };
+        unsigned cut = 0;
+        // no id, or not enough mass even at the end: nothing is cut
+        const bool some = b1 < BUCKETS;
+        bool sure = !some || (total <= LIST && !(b1 > 0 && enough(above_n, above_w)));
+        if (some && sure) {
+            if (rank == 0) {
+                // rank 0 gathers the list behind its own, and looks for the largest key down to which k ids, or the mass, are there
+                for (int q = 1, base = s.listed; q < cs; ++q) {
+                    const int other = *at(&s.listed, q);
+                    const unsigned* keys = at(s.list_key, q);
+                    const u64* ws = at(s.list_w, q);
+                    for (int i = tid; i < other; i += RT) { s.list_key[base + i] = keys[i]; s.list_w[base + i] = ws[i]; }
+                    base += other;
+                }
+                __syncthreads();
+                if (total <= kPairs) {
+                    // each with each; all of a tie write the same
+                    const unsigned key = tid < total ? s.list_key[tid] : 0;
+                    unsigned ge = above_n, gt = above_n;
+                    u64 wge = above_w, wgt = above_w;
+                    for (int j = 0; j < total; ++j) {
+                        const unsigned k = s.list_key[j];
+                        const u64 x = s.list_w[j];
+                        if (k >= key) { ++ge; wge += x; }
+                        if (k > key) { ++gt; wgt += x; }
+                    }
+                    if (tid < total && enough(ge, wge) && (gt == 0 || !enough(gt, wgt)))
+                        for (int q = 0; q < cs; ++q) { *at(&s.cut, q) = key; *at(&s.found, q) = 1; }
+                } else {
+                    // by the bits in which they differ
+                    constexpr int EACH = LIST / RT;
+                    unsigned key[EACH], most = 0, least = 0xffffffffu;
+                    u64 x[EACH];
+#pragma unroll
+                    for (int e = 0; e < EACH; ++e) {
+                        const int i = tid + e * RT;
+                        key[e] = i < total ? s.list_key[i] : 0;
+                        x[e] = i < total ? s.list_w[i] : 0;
+                        most = max(most, key[e]);
+                        least = min(least, i < total ? key[e] : 0xffffffffu);
+                    }
+                    most = __reduce_max_sync(0xffffffffu, most);
+                    least = __reduce_min_sync(0xffffffffu, least);
+                    if (lane == 0) { s.warp_n[warp] = most; s.pair_n[0][warp] = least; }
+                    __syncthreads();
+                    for (int q = 0; q < RW; ++q) { most = max(most, s.warp_n[q]); least = min(least, s.pair_n[0][q]); }
+                    __syncthreads();
+                    const int bits = 32 - __clz(most ^ least);
+                    unsigned c = bits < 32 ? most >> bits << bits : 0;
+                    bool reached = false;
+                    for (int bit = bits; bit >= 0; --bit) {           // (first what they have in common)
+                        const unsigned cand = bit == bits ? c : c | 1u << bit;
+                        unsigned n = 0;
+                        u64 w = 0;
+#pragma unroll
+                        for (int e = 0; e < EACH; ++e)
+                            if (key[e] >= cand && tid + e * RT < total) { ++n; w += x[e]; }
+                        n = __reduce_add_sync(0xffffffffu, n);
+                        w = warp_sum(w);
+                        if (lane == 0) { s.pair_n[bit & 1][warp] = n; s.pair_w[bit & 1][warp] = w; }
+                        __syncthreads();
+                        n = above_n; w = above_w;
+                        for (int q = 0; q < RW; ++q) { n += s.pair_n[bit & 1][q]; w += s.pair_w[bit & 1][q]; }
+                        if (enough(n, w)) { c = cand; reached = true; }
+                    }
+                    if (tid == 0 && reached)
+                        for (int q = 0; q < cs; ++q) { *at(&s.cut, q) = c; *at(&s.found, q) = 1; }
+                }
+            }
+            sync();
+            sure = s.found != 0;
+            // not in the list though the buckets end behind it: the mass is never reached, and nothing is cut
+            if (!sure && s.b2 == BUCKETS) sure = true;
+            else cut = sure ? s.cut : 0;
+        }
+        if (!sure) {
+            // the cut's bits from the highest down, a pass each over what is not above those buckets
+            struct Count {
+                const Weigher& weigh;
+                const decltype(bucket_of)& bucket;
+                int from;
+                unsigned cand;
+                bool mass_too;
+                unsigned& n;
+                u64& w;
+                __device__ __forceinline__ void operator()(const float (&v)[4], int) const {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (v[e] > -INFINITY && logit_key(v[e]) >= cand && bucket(v[e]) >= from) {
+                            ++n;
+                            if (mass_too && v[e] >= weigh.least) w += weigh.fixed(v[e]);
+                        }
+                }
+                __device__ __forceinline__ void done(int) const {}
+            };
+            const bool before = b1 > 0 && enough(above_n, above_w);       // (the f32 masses were wrong: from the start)
+            cut = 0;
+            for (int bit = 31; bit >= 0; --bit) {
+                const unsigned cand = cut | (1u << bit);
+                unsigned n = 0;
+                u64 w = 0;
+                ids.over(Count{weigh, bucket_of, before ? 0 : b1, cand, cut_p, n, w});
+                n = __reduce_add_sync(0xffffffffu, n);
+                w = warp_sum(w);
+                __syncthreads();
+                if (lane == 0) { s.warp_n[warp] = n; s.warp_w[warp] = w; }
+                __syncthreads();
+                if (tid == 0) {
+                    for (int q = 1; q < RW; ++q) { n += s.warp_n[q]; w += s.warp_w[q]; }
+                    s.wide_n = n; s.wide_w = w;
+                }
+                sync();
+                n = 0; w = 0;
+                for (int q = 0; q < cs; ++q) { n += *at(&s.wide_n, q); w += *at(&s.wide_w, q); }
+                if (n && enough(before ? n : above_n + n, before ? w : above_w + w)) cut = cand;
+                sync();
+            }
+            if (cut) keep = fmaxf(keep, key_logit(cut));
+            ids.over(Keep{s, weigh, keep, lane, lane_sum, warp_all});
+        } else {
+            if (cut) keep = fmaxf(keep, key_logit(cut));
+            // what stays of the list joins its chunks
+            __syncthreads();
+            const int mine = min(s.listed, LIST);
+            for (int i = tid; i < mine; i += RT)
+                if (key_logit(s.list_key[i]) >= keep) atomicAdd(&s.chunk[s.list_chunk[i]], s.list_w[i]);
+            __syncthreads();
+            const int chunks = (end - begin + chunk - 1) / chunk;
+            for (int i = tid; i < chunks; i += RT) lane_sum += s.chunk[i];
+            warp_all = warp_sum(lane_sum);
+        }
+        __syncthreads();                      // the warps' sums of the pass have been read
     }
-    __syncthreads();                          // the warps' sums of the buckets have been read
     if (lane == 0) s.warp_w[warp] = warp_all;
     __syncthreads();
     if (tid == 0) {
@@ -459,10 +603,8 @@ __global__ void __launch_bounds__(RT, 2) sample_rows_kernel(const float* __restr
         }
         const int per_lane = chunk / 32, i0 = begin + c0 * chunk + lane * per_lane, i1 = min(i0 + per_lane, end);
         auto weight = [&](int i) -> u64 {
-            const float l = row.fix(__ldg(row.p + i));
-            if (!(l >= weigh.least) || logit_key(l) < cut) return 0;
-            const double x = weigh.log2w(l);
-            return x >= floor_x ? weigh.fixed(x) : 0;
+            const float l = ids.at(i);
+            return l >= keep ? weigh.fixed(l) : 0;
         };
         u64 w = 0;
         for (int i = i0; i < i1; ++i) w += weight(i);
@@ -481,7 +623,7 @@ __global__ void __launch_bounds__(RT, 2) sample_rows_kernel(const float* __restr
                 if (there(m)) break;
             }
             token[r] = i;
-            if (prob) prob[r] = (float)(weigh.exact(weigh.log2w(row.fix(__ldg(row.p + i)))) * (double)(1ull << kFix) / (double)whole);
+            if (prob) prob[r] = (float)(weigh.exact(ids.at(i)) * (double)(1ull << kFix) / (double)whole);
         }
     }
     if (cs > 1) cluster.sync();               // no rank leaves while another reads its memory
@@ -502,21 +644,23 @@ extern "C" int fc_sample_rows_dev(int device, const float* logits, int64_t ld, i
     static bool ready[64] = {};
     if (device < 0 || device >= 64 || !ready[device]) {
         FC_TRY(select_device(device));
-        FC_CUDA(cudaFuncSetAttribute(sample_rows_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(Shared)));
+        FC_CUDA(cudaFuncSetAttribute(sample_rows_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(Shared) + kSlice * sizeof(float)));
         if (device < 64) ready[device] = true;
     } else {
         int current = -1;
         FC_CUDA(cudaGetDevice(&current));
         if (current != device) FC_CUDA(cudaSetDevice(device));
     }
-    // as many CTAs a row as are resident, each with 2048 ids at least
+    // a CTA costs some microseconds whatever it holds: no more of them than are resident, 1024 ids each at least
     int cs = 1, chunk = 128;
-    while (cs < 8 && (long long)n_rows * cs * 2 <= 148 * 3 && (long long)cs * 2 * 2048 <= vocab) cs *= 2;
+    while (cs < 8 && (long long)n_rows * cs * 2 <= 148 * 3 && (long long)cs * 2 * 1024 <= vocab) cs *= 2;
     while ((vocab + cs - 1) / cs > chunk * (CHUNKS - 1)) chunk *= 2;
+    const int share = ((vocab + cs - 1) / cs + chunk - 1) / chunk * chunk;
+    const bool in_shared = share <= kSlice && (share <= kSlice / 8 || (long long)n_rows * cs <= 148);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)n_rows * cs);
     cfg.blockDim = dim3(RT);
-    cfg.dynamicSmemBytes = sizeof(Shared);
+    cfg.dynamicSmemBytes = sizeof(Shared) + (in_shared ? (size_t)share * sizeof(float) : 0);
     cfg.stream = (cudaStream_t)stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -524,7 +668,7 @@ extern "C" int fc_sample_rows_dev(int device, const float* logits, int64_t ld, i
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    FC_CUDA(cudaLaunchKernelEx(&cfg, sample_rows_kernel, logits, (long long)ld, vocab, params, u, token, prob, cs, chunk));
+    FC_CUDA(cudaLaunchKernelEx(&cfg, sample_rows_kernel, logits, (long long)ld, vocab, params, u, token, prob, cs, chunk, (int)in_shared));
     FC_LAUNCHED();
     return FC_OK;
 }
