@@ -70,9 +70,14 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(Kv4 c, const int* __restr
                 for (int g = 0; g < 8; ++g) x[g] = d * (float)((int)(w >> (4 * g) & 15) - 8);
             }
         }
-        float4* to = (float4*)((values ? v : k) + ((((size_t)seq * n + i) * c.n_kv + h) * parts + part) * 8);
-        to[0] = make_float4(x[0], x[1], x[2], x[3]);
-        to[1] = make_float4(x[4], x[5], x[6], x[7]);
+        // two lanes exchange halves, so that a store writes whole lines: the even lane's channels first, then the odd one's
+        const bool odd = threadIdx.x & 1;
+        float y[4];
+#pragma unroll
+        for (int g = 0; g < 4; ++g) y[g] = __shfl_xor_sync(3u << (threadIdx.x & 30), odd ? x[g] : x[4 + g], 1);
+        float4* to = (float4*)((values ? v : k) + ((((size_t)seq * n + i) * c.n_kv + h) * parts + (part & ~1)) * 8) + odd;
+        to[0] = odd ? make_float4(y[0], y[1], y[2], y[3]) : make_float4(x[0], x[1], x[2], x[3]);
+        to[2] = odd ? make_float4(x[4], x[5], x[6], x[7]) : make_float4(y[0], y[1], y[2], y[3]);
     }
 }
 
@@ -114,7 +119,7 @@ __global__ void __launch_bounds__(ET, 2) kv4_evict_kernel(Kv4 src, Kv4 dst, cons
     const int old = all ? 0 : len - recent, want = budget - recent;      // of the first `old` positions the `want` heaviest
     const bool fits = old <= KEYS;
     if (fits)
-#pragma unroll 4
+#pragma unroll 16
         for (int j = tid; j < old; j += ET) s.key[j] = weight_key(__ldg(m + j));
     auto key = [&](int j) { return fits ? s.key[j] : weight_key(__ldg(m + j)); };
     unsigned cut = 0;
@@ -128,7 +133,7 @@ __global__ void __launch_bounds__(ET, 2) kv4_evict_kernel(Kv4 src, Kv4 dst, cons
             __syncthreads();
             const unsigned high = pass ? cut >> (shift + width) : 0, mask = (1u << width) - 1;
             if (pass == 0) {
-#pragma unroll 4
+#pragma unroll 8
                 for (int j = tid; j < old; j += ET) atomicAdd(&s.bins[key(j) >> shift], 1u);
             } else if (pass == 1) {
                 // the keys of the first digit's bin, listed where they fit
@@ -188,6 +193,7 @@ __global__ void __launch_bounds__(ET, 2) kv4_evict_kernel(Kv4 src, Kv4 dst, cons
     const int per = ((old + ET - 1) / ET) | 1, j0 = min(old, tid * per), j1 = min(old, j0 + per);
     int sure = 0, tie = 0;
     if (want > 0)
+#pragma unroll 8
         for (int j = j0; j < j1; ++j) {
             const unsigned k = key(j);
             sure += k > cut;

@@ -20,7 +20,7 @@ class Kv4Cache:
         self.n_seq, self.n_kv_head, self.head_dim, self.capacity, self.device = n_seq, n_kv_head, head_dim, capacity, device
         L = _lib.lib()
         check(L.fc_kv4_create(device, n_seq, n_kv_head, head_dim, capacity, C.byref(self._h)))
-        self._attend, self._read = L.fc_kv4_attend_dev, L.fc_kv4_read_dev      # a short step takes less time than two lookups
+        self._attend, self._read, self._evict = L.fc_kv4_attend_dev, L.fc_kv4_read_dev, L.fc_kv4_evict_dev   # a short step takes less time than two lookups
 
     def _rows(self, rows):
         if rows is None or isinstance(rows, C.Array):
@@ -49,7 +49,9 @@ class Kv4Cache:
 
     def evict_dev(self, dst, lens_ptr, lens_out_ptr, budget, recent, mass_ptr, mass_out_ptr=None, kept_ptr=None, stream=None):
         """The last `recent` positions and the heaviest others, `budget` in all, to the cache `dst`."""
-        check(_lib.lib().fc_kv4_evict_dev(self._h, dst._h, lens_ptr, lens_out_ptr, budget, recent, mass_ptr, mass_out_ptr, kept_ptr, stream))
+        rc = self._evict(self._h, dst._h, lens_ptr, lens_out_ptr, budget, recent, mass_ptr, mass_out_ptr, kept_ptr, stream)
+        if rc:
+            check(rc)
 
     def close(self):
         if self._h:
