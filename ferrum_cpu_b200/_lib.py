@@ -136,6 +136,8 @@ SIGNATURES = {
     "fc_llama_score_sequences": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.POINTER(FcScore), C.c_void_p]),
     "fc_llama_last_score_ms": (C.c_float, [C.c_void_p]),
     "fc_llama_cache_create": (C.c_int, [C.c_void_p, C.POINTER(C.c_void_p)]),
+    "fc_llama_cache_create_kv4": (C.c_int, [C.c_void_p, C.c_int, C.c_int, C.c_int, C.POINTER(C.c_void_p)]),
+    "fc_llama_cache_held": (C.c_int, [C.c_void_p]),
     "fc_llama_cache_free": (None, [C.c_void_p]),
     "fc_llama_cache_clear": (C.c_int, [C.c_void_p]),
     "fc_llama_cache_pos": (C.c_int, [C.c_void_p]),

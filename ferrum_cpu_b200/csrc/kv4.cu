@@ -273,6 +273,38 @@ int launch_kv4_append(const Kv4& c, const float* k, const float* v, int ldkv, co
     return FC_OK;
 }
 
+int kv4_make(Arena& arena, int n_seq, int n_kv, int dim, int cap, Kv4* c) {
+    const int pad = (cap + kKvTile - 1) / kKvTile * kKvTile;
+    const size_t rows = (size_t)n_seq * n_kv * pad, q = rows * dim / 2, d = rows * (dim / kKvBlock) * 2;
+    *c = Kv4{nullptr, nullptr, nullptr, nullptr, n_seq, n_kv, dim / kKvBlock, cap, pad};
+    FC_TRY(arena.alloc((void**)&c->kq, q));
+    FC_TRY(arena.alloc((void**)&c->vq, q));
+    FC_TRY(arena.alloc((void**)&c->kd, d));
+    FC_TRY(arena.alloc((void**)&c->vd, d));
+    FC_CUDA(cudaMemset(c->kq, 0, q));
+    FC_CUDA(cudaMemset(c->vq, 0, q));
+    FC_CUDA(cudaMemset(c->kd, 0, d));
+    FC_CUDA(cudaMemset(c->vd, 0, d));
+    FC_CUDA(cudaDeviceSynchronize());
+    return FC_OK;
+}
+
+int launch_kv4_evict(const Kv4& a, const Kv4& b, const int* lens, int* lens_out, int budget, int recent, const float* mass, float* mass_out, int* kept, int device,
+                     cudaStream_t st) {
+    static bool attr_set[64] = {};
+    if (device >= 64 || !attr_set[device]) {
+        FC_CUDA(cudaFuncSetAttribute(kv4_evict_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(EvictShared)));
+        if (device < 64) attr_set[device] = true;
+    }
+    // CTAs that share a head: as many as are resident, 64 rows of dst each at least
+    const long long heads = (long long)a.n_kv * a.n_seq;
+    int share = 1;
+    while (share < 32 && heads * share * 2 <= 296 && budget >= share * 2 * 64) share *= 2;
+    kv4_evict_kernel<<<dim3(share, a.n_kv, a.n_seq), ET, sizeof(EvictShared), st>>>(a, b, lens, lens_out, budget, recent, mass, mass_out, kept);
+    FC_LAUNCHED();
+    return FC_OK;
+}
+
 int make_device(int device) {
     // asking is cheaper than setting, and nearly every call finds its device current
     int current = -1;
@@ -315,22 +347,7 @@ int fc_kv4_create(int device, int n_seq, int n_kv_head, int head_dim, int capaci
     FC_TRY(scratch_retain(device));
     fc_kv4* c = new fc_kv4();
     c->device = device;
-    auto build = [&]() -> int {
-        const int pad = (capacity + kKvTile - 1) / kKvTile * kKvTile;
-        const size_t rows = (size_t)n_seq * n_kv_head * pad, q = rows * head_dim / 2, d = rows * (head_dim / kKvBlock) * 2;
-        c->c = Kv4{nullptr, nullptr, nullptr, nullptr, n_seq, n_kv_head, head_dim / kKvBlock, capacity, pad};
-        FC_TRY(c->arena.alloc((void**)&c->c.kq, q));
-        FC_TRY(c->arena.alloc((void**)&c->c.vq, q));
-        FC_TRY(c->arena.alloc((void**)&c->c.kd, d));
-        FC_TRY(c->arena.alloc((void**)&c->c.vd, d));
-        FC_CUDA(cudaMemset(c->c.kq, 0, q));
-        FC_CUDA(cudaMemset(c->c.vq, 0, q));
-        FC_CUDA(cudaMemset(c->c.kd, 0, d));
-        FC_CUDA(cudaMemset(c->c.vd, 0, d));
-        FC_CUDA(cudaDeviceSynchronize());
-        return FC_OK;
-    };
-    const int rc = build();
+    const int rc = kv4_make(c->arena, n_seq, n_kv_head, head_dim, capacity, &c->c);
     if (rc != FC_OK) { fc_kv4_free(c); return rc; }
     *out = c;
     return FC_OK;
@@ -401,18 +418,7 @@ int fc_kv4_evict_dev(const fc_kv4* src, fc_kv4* dst, const int32_t* lens, int32_
     if (budget <= 0 || recent < 0 || recent > budget) return fail(FC_E_SHAPE, "fc_kv4_evict_dev: budget %d, recent %d", budget, recent);
     if (budget > b.cap) return fail(FC_E_DIM, "fc_kv4_evict_dev: a budget of %d does not fit %d positions", budget, b.cap);
     FC_TRY(make_device(src->device));
-    static bool attr_set[64] = {};
-    if (src->device >= 64 || !attr_set[src->device]) {
-        FC_CUDA(cudaFuncSetAttribute(kv4_evict_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(EvictShared)));
-        if (src->device < 64) attr_set[src->device] = true;
-    }
-    // CTAs that share a head: as many as are resident, 64 rows of dst each at least
-    const long long heads = (long long)a.n_kv * a.n_seq;
-    int share = 1;
-    while (share < 32 && heads * share * 2 <= 296 && budget >= share * 2 * 64) share *= 2;
-    kv4_evict_kernel<<<dim3(share, a.n_kv, a.n_seq), ET, sizeof(EvictShared), (cudaStream_t)stream>>>(a, b, lens, lens_out, budget, recent, mass, mass_out, kept);
-    FC_LAUNCHED();
-    return FC_OK;
+    return launch_kv4_evict(a, b, lens, lens_out, budget, recent, mass, mass_out, kept, src->device, (cudaStream_t)stream);
 }
 
 }  // extern "C"

@@ -9,6 +9,7 @@
 #include "llama_native.h"
 #include <climits>
 
+#include "kv4_ops.cuh"
 #include "llama_ops.cuh"
 
 using namespace fc;
@@ -61,11 +62,27 @@ struct fc_llama {
     fc_ggml_weight* native_tok = nullptr;   // the embedding table in its block format (kNative)
 };
 
+// The keys and values of a cache in 4-bit levels (kv4.cuh): `cap` positions a layer. With fewer positions than the context, a cache that has
+// run full is cut down to `budget` positions: their rows move from one set of layers to the other, which the next steps then use.
+struct LlamaKv4 {
+    bool on = false;
+    int cap = 0, budget = 0, recent = 0;
+    std::vector<Kv4> layers[2];
+    float* mass[2] = {nullptr, nullptr};  // [L][n_kv][cap], where positions are evicted
+    int* words = nullptr;                 // positions held by either set, 0, ids of the prompt
+    Kv4 prompt{};                         // one layer's rows of a prompt that is longer than `cap`, and their weights; made when the first comes
+    float* prompt_mass = nullptr;
+    int set = 0, held = 0;
+    bool evicts() const { return mass[0] != nullptr; }
+};
+
 struct fc_llama_cache {
     fc_llama* m = nullptr;
     int device = 0;                       // kept here so that freeing does not read the model
     Arena arena;
-    float *kc = nullptr, *vc = nullptr;   // [L][ctx][kv_dim]
+    float *kc = nullptr, *vc = nullptr;   // [L][ctx][kv_dim]; null: kv4
+    LlamaKv4 kv4;
+    bool scratch = false;                 // the device's pool is kept for this cache
     float *x = nullptr, *n = nullptr, *qkv = nullptr, *att = nullptr, *gu = nullptr, *hid = nullptr, *logits = nullptr;
     int* queue = nullptr;
     int queue_cap = 0;
@@ -174,6 +191,27 @@ int ensure_workspace(fc_llama* m, int rows) {
     return FC_OK;
 }
 
+// Attention of R rotated rows of a fused q | k | v buffer over a 4-bit cache that holds *len positions; the rows join it.
+int attend_kv4(fc_llama* m, const Kv4& c, const float* qkv, int R, const int* len, float* mass, float* att) {
+    const fc_llama_config& g = m->cfg;
+    const Kv4Attend a = {qkv, qkv + m->q_dim, qkv + m->q_dim + m->kv_dim, att, m->qkv_dim, m->qkv_dim, m->q_dim, g.n_head / g.n_kv_head,
+                         1.0f / std::sqrt((float)g.head_dim), len, mass};
+    KvRows rows;
+    rows.start[0] = 0;
+    rows.start[1] = R;
+    return launch_kv4_attend(c, a, rows, R, m->device, m->st);
+}
+size_t kv4_layer_mass(const fc_llama_cache* s) { return (size_t)s->m->cfg.n_kv_head * s->kv4.cap; }
+// Block l of a prompt of R rows, in an empty cache: straight into the layer, or by way of the prompt's own rows when they do not fit.
+int prompt_kv4(fc_llama_cache* s, int l, const float* qkv, int R, float* att) {
+    LlamaKv4& k = s->kv4;
+    fc_llama* m = s->m;
+    float* mass = k.evicts() ? k.mass[k.set] + l * kv4_layer_mass(s) : nullptr;
+    if (R <= k.cap) return attend_kv4(m, k.layers[k.set][l], qkv, R, k.words + 2, mass, att);
+    FC_TRY(attend_kv4(m, k.prompt, qkv, R, k.words + 2, k.prompt_mass, att));
+    return launch_kv4_evict(k.prompt, k.layers[k.set][l], k.words + 3, k.words + k.set, k.budget, k.recent, k.prompt_mass, mass, nullptr, m->device, m->st);
+}
+
 // LlamaModel::forward_tokens (llm.rs:622-635) up to the final norm, for B windows of T rows
 // whose ids are in m->ids_d: every row r sits at position r % T. Leaves RMSNorm(h) in m->n
 // and, for the Q8_0 model, its planes in m->px.
@@ -204,14 +242,19 @@ int forward_rows(fc_llama* m, int B, int T, fc_llama_cache* fill = nullptr) {
         } else {
             FC_TRY(launch_llama_rope_rows(m->qkv, R, m->qkv_dim, T, c.n_head, c.n_kv_head, m->q_dim, c.head_dim, c.rope_dim,
                                           c.rope_type == FC_ROPE_NEOX, m->ftab, m->inv_linear, st));
-            if (tc_attn) FC_TRY(launch_split_planes(m->qkv, m->pqkv, (size_t)R * m->qkv_dim, st));
+            if (tc_attn && !(fill && fill->kv4.on)) FC_TRY(launch_split_planes(m->qkv, m->pqkv, (size_t)R * m->qkv_dim, st));
         }
-        if (fill) {
+        if (fill && fill->kv4.on) {
+            FC_TRY(prompt_kv4(fill, l, m->qkv, R, m->att));
+            FC_TRY(launch_split_planes(m->att, m->patt, (size_t)R * m->q_dim, st));
+        } else if (fill) {
             const size_t layer_stride = (size_t)c.ctx * m->kv_dim;
             FC_TRY(launch_llama_store_kv_rows(m->qkv, R, m->qkv_dim, m->q_dim, m->kv_dim, fill->kc + l * layer_stride,
                                               fill->vc + l * layer_stride, st));
         }
-        if (tc_attn) {
+        if (fill && fill->kv4.on) {
+            // (attended above)
+        } else if (tc_attn) {
             FC_TRY(launch_attn_prefill_tc_gqa(m->pqkv, win, R, c.n_head, c.n_kv_head, m->patt, m->tc_status, st));
         } else {
             FC_TRY(launch_attn_prefill_gqa(m->qkv, m->qkv + m->q_dim, m->qkv + m->q_dim + m->kv_dim, win, m->qkv_dim, c.n_head,
@@ -285,6 +328,7 @@ int forward_rows_packed(fc_llama* m, int B, int T, fc_llama_cache* fill) {
         FC_TRY(packed_block(m, l, R, m->x, m->n, m->qkv, m->att, m->gu, m->hid, nullptr, [&]() -> int {
             FC_TRY(launch_llama_rope_rows(m->qkv, R, m->qkv_dim, T, c.n_head, c.n_kv_head, m->q_dim, c.head_dim, c.rope_dim,
                                           c.rope_type == FC_ROPE_NEOX, m->ftab, m->inv_linear, st));
+            if (fill && fill->kv4.on) return prompt_kv4(fill, l, m->qkv, R, m->att);
             if (fill) {
                 const size_t layer_stride = (size_t)c.ctx * m->kv_dim;
                 FC_TRY(launch_llama_store_kv_rows(m->qkv, R, m->qkv_dim, m->q_dim, m->kv_dim, fill->kc + l * layer_stride,
@@ -355,14 +399,34 @@ int check_window(const fc_llama* m, int window) {
     return FC_OK;
 }
 
-int launch_attention(fc_llama_cache* s, float* kc, float* vc, int split) {
+int launch_attention(fc_llama_cache* s, int l, int split) {
     fc_llama* m = s->m;
     const fc_llama_config& c = m->cfg;
+    if (s->kv4.on) {
+        const LlamaKv4& k = s->kv4;
+        FC_TRY(launch_llama_rope_step(s->qkv, c.n_head, c.n_kv_head, m->q_dim, c.head_dim, c.rope_dim, c.rope_type == FC_ROPE_NEOX, m->ftab, m->inv_linear,
+                                      s->state, m->st));
+        return attend_kv4(m, k.layers[k.set][l], s->qkv, 1, k.words + k.set, k.evicts() ? k.mass[k.set] + l * kv4_layer_mass(s) : nullptr, s->att);
+    }
+    const size_t layer_stride = (size_t)c.ctx * m->kv_dim;
+    float *kc = s->kc + l * layer_stride, *vc = s->vc + l * layer_stride;
     if (attn_step_covers(c.head_dim, c.ctx))
         return launch_attn_step(s->qkv, c.n_head, c.n_kv_head, c.head_dim, c.rope_dim, c.rope_type == FC_ROPE_NEOX, m->ftab, m->inv_linear,
                                 kc, vc, c.ctx, split, s->state, s->att, m->st);
     return launch_llama_attn_decode(s->qkv, c.n_head, c.n_kv_head, c.head_dim, c.rope_dim, c.rope_type == FC_ROPE_NEOX, m->ftab, m->inv_linear,
                                     kc, vc, c.ctx, s->state, s->att, m->st);
+}
+
+// A step that was not given up: the cache holds a position more.
+__global__ void llama_kv4_held_kernel(const StepState* st, int* held) {
+    if (!(st->done | st->error)) *held += 1;
+}
+int end_step(fc_llama_cache* s) {
+    if (s->kv4.on) {
+        llama_kv4_held_kernel<<<1, 1, 0, s->m->st>>>(s->state, s->kv4.words + s->kv4.set);
+        FC_LAUNCHED();
+    }
+    return launch_step_advance_pdl(s->state, s->m->st);
 }
 
 // ---------------------------------------------------------------------------- decode step
@@ -439,22 +503,19 @@ int launch_step(fc_llama_cache* s, int with_head, int split) {
     fc_llama* m = s->m;
     const fc_llama_config& c = m->cfg;
     cudaStream_t st = m->st;
-    const size_t layer_stride = (size_t)c.ctx * m->kv_dim;
     FC_TRY(launch_llama_embed_step(m->tok, c.ctx, s->queue, s->state, s->x, st));
     for (int l = 0; l < c.n_layer; ++l) {
         const LlamaLayerDev& L = m->layers[l];
-        float* kc = s->kc + l * layer_stride;
-        float* vc = s->vc + l * layer_stride;
         // RMSNorm rides in the prologue of the projection that reads it, SwiGLU in the epilogue of gate/up
         FC_TRY(launch_gemv_row(L.qkv, s->x, RowNorm{L.attn_norm, nullptr, c.norm_eps}, L.qkv_b, nullptr, EPI_NONE, s->qkv, s->state, st));
-        FC_TRY(launch_attention(s, kc, vc, split));
+        FC_TRY(launch_attention(s, l, split));
         FC_TRY(launch_gemv_row(L.wo, s->att, RowNorm(), nullptr, s->x, EPI_NONE, s->x, s->state, st));
         FC_TRY(launch_gemv_row(L.gateup, s->x, RowNorm{L.ffn_norm, nullptr, c.norm_eps}, nullptr, nullptr, EPI_SWIGLU, s->hid, s->state, st));
         FC_TRY(launch_gemv_row(L.down, s->hid, RowNorm(), nullptr, s->x, EPI_NONE, s->x, s->state, st));
     }
     if (with_head)
         FC_TRY(launch_gemv_row(m->head, s->x, RowNorm{m->out_norm, nullptr, c.norm_eps}, nullptr, nullptr, EPI_NONE, s->logits, s->state, st));
-    return launch_step_advance_pdl(s->state, st);
+    return end_step(s);
 }
 
 // The same step on the packed model, one kernel per operation. The first step of a cache runs uncaptured, so that the
@@ -464,12 +525,9 @@ int launch_step_packed(fc_llama_cache* s, int with_head, int split) {
     fc_llama* m = s->m;
     const fc_llama_config& c = m->cfg;
     cudaStream_t st = m->st;
-    const size_t layer_stride = (size_t)c.ctx * m->kv_dim;
     if (m->native_tok) FC_TRY(launch_ggml_rows(m->native_tok, nullptr, s->state, s->queue, c.ctx, 1, s->x, nullptr, st));
     else FC_TRY(launch_llama_embed_step(m->tok, c.ctx, s->queue, s->state, s->x, st));
     for (int l = 0; l < c.n_layer; ++l) {
-        float* kc = s->kc + l * layer_stride;
-        float* vc = s->vc + l * layer_stride;
         const fc_llama::PackedLayer& P = m->packed[l];
         const LlamaLayerDev& L = m->layers[l];
         const float* b = L.qkv_b;
@@ -480,14 +538,14 @@ int launch_step_packed(fc_llama_cache* s, int with_head, int split) {
             rowq_part(P.up.rq, nullptr, s->hid, &gu[1]) && rowq_part(P.down.rq, nullptr, s->x, &down)) {
             // five kernels, as the Q8_0 step: the norms are prologues, SwiGLU and the residual epilogues
             FC_TRY(launch_gemv_row(in, 3, c.d_model, s->x, RowNorm{L.attn_norm, nullptr, c.norm_eps}, nullptr, EPI_NONE, s->state, st));
-            FC_TRY(launch_attention(s, kc, vc, split));
+            FC_TRY(launch_attention(s, l, split));
             FC_TRY(launch_gemv_row(&wo, 1, m->q_dim, s->att, RowNorm(), s->x, EPI_NONE, s->state, st));
             FC_TRY(launch_gemv_row(gu, 2, c.d_model, s->x, RowNorm{L.ffn_norm, nullptr, c.norm_eps}, nullptr, EPI_SWIGLU, s->state, st));
             FC_TRY(launch_gemv_row(&down, 1, c.d_ff, s->hid, RowNorm(), s->x, EPI_NONE, s->state, st));
             continue;
         }
         FC_TRY(packed_block(m, l, 1, s->x, s->n, s->qkv, s->att, s->gu, s->hid, nullptr, [&]() -> int {
-            return launch_attention(s, kc, vc, split);
+            return launch_attention(s, l, split);
         }));
     }
     if (with_head) {
@@ -499,7 +557,7 @@ int launch_step_packed(fc_llama_cache* s, int with_head, int split) {
             FC_TRY(lin_apply(m, m->packed_head, s->n, nullptr, nullptr, s->logits, m->head.N_pad, 1));
         }
     }
-    return launch_step_advance_pdl(s->state, st);
+    return end_step(s);
 }
 
 // Greedy tokens that need nothing from the host share a graph: between two graphs the GPU waits for the next one's launch.
@@ -513,9 +571,22 @@ void drop_graphs(fc_llama_cache* s) {
         }
 }
 
-// pos: the position of the (first) step
+// Room for n more positions in a 4-bit cache that evicts.
+int make_room(fc_llama_cache* s, int n) {
+    LlamaKv4& k = s->kv4;
+    if (!k.on || !k.evicts() || k.held + n <= k.cap) return FC_OK;
+    const int from = k.set, to = 1 - k.set;
+    for (int l = 0; l < s->m->cfg.n_layer; ++l)
+        FC_TRY(launch_kv4_evict(k.layers[from][l], k.layers[to][l], k.words + from, k.words + to, k.budget, k.recent, k.mass[from] + l * kv4_layer_mass(s),
+                                k.mass[to] + l * kv4_layer_mass(s), nullptr, s->m->device, s->m->st));
+    k.set = to;
+    k.held = std::min(k.held, k.budget);
+    return FC_OK;
+}
+
+// pos: the position of the (first) step. A 4-bit cache has its graphs by the set of layers that they use.
 int run_graph(fc_llama_cache* s, int which, int pos) {
-    const bool shared = pos + (which == 2 ? kFreeSteps : 1) > s->split_from;
+    const bool shared = s->kv4.on ? s->kv4.set == 1 : pos + (which == 2 ? kFreeSteps : 1) > s->split_from;
     if (s->graph_wait != g_debug.wait_cycles || s->graph_withhold != g_debug.withhold) {
         FC_CUDA(cudaStreamSynchronize(s->m->st));
         drop_graphs(s);
@@ -560,6 +631,11 @@ int run_step(fc_llama_cache* s, int with_head, int pos) {
     return run_graph(s, with_head, pos);
 }
 
+__global__ void llama_set_words_kernel(int* words, int set, int held, int prompt) {
+    words[set] = held;
+    words[2] = 0;
+    words[3] = prompt;
+}
 __global__ void llama_set_state_kernel(StepState* st, int pos, int fed, int tail) {
     st->pos = pos; st->fed = fed; st->tail = tail; st->done = 0; st->eos = -1; st->error = 0;
 }
@@ -574,6 +650,7 @@ int read_state(fc_llama_cache* s, StepState* out) {
 int step_error(fc_llama_cache* s, const StepState& hs) {
     if (!hs.error) return FC_OK;
     s->host_pos = std::min(s->host_pos, hs.pos);
+    if (s->kv4.on) FC_CUDA(cudaMemcpy(&s->kv4.held, s->kv4.words + s->kv4.set, sizeof(int), cudaMemcpyDeviceToHost));
     return fail(hs.error, hs.error == FC_E_TIMEOUT ? "a bounded wait inside a decode step ran out" : "the decode step rejected a token or position on the device");
 }
 
@@ -585,7 +662,11 @@ int feed_ids(fc_llama_cache* s, const int32_t* ids, int n, int head_on_last) {
     FC_CUDA(cudaMemcpyAsync(s->queue + s->host_pos, ids, (size_t)n * 4, cudaMemcpyHostToDevice, m->st));
     llama_set_state_kernel<<<1, 1, 0, m->st>>>(s->state, s->host_pos, s->host_pos, s->host_pos + n);
     FC_LAUNCHED();
-    for (int i = 0; i < n; ++i) FC_TRY(run_step(s, head_on_last && i + 1 == n, s->host_pos + i));
+    for (int i = 0; i < n; ++i) {
+        FC_TRY(make_room(s, 1));
+        FC_TRY(run_step(s, head_on_last && i + 1 == n, s->host_pos + i));
+        s->kv4.held += 1;
+    }
     s->host_pos += n;
     return FC_OK;
 }
@@ -599,6 +680,15 @@ int prime_window(fc_llama_cache* s, const int32_t* ids, int n) {
     const fc_llama_config& c = m->cfg;
     if (n > c.ctx) return fail(FC_E_DIM, "%d tokens do not fit the model's %d-token context window", n, c.ctx);
     cudaStream_t st = m->st;
+    LlamaKv4& k = s->kv4;
+    if (k.on && n > k.cap && !k.prompt.kq) {
+        FC_TRY(s->arena.alloc_n(&k.prompt_mass, (size_t)c.n_kv_head * c.ctx));
+        FC_TRY(kv4_make(s->arena, 1, c.n_kv_head, c.head_dim, c.ctx, &k.prompt));
+    }
+    if (k.on) {
+        llama_set_words_kernel<<<1, 1, 0, st>>>(k.words, k.set, 0, n);
+        FC_LAUNCHED();
+    }
     m->force_fp32 = true;
     int rc = ensure_workspace(m, n);
     if (rc == FC_OK && cudaMemcpyAsync(m->ids_d, ids, (size_t)n * 4, cudaMemcpyHostToDevice, st) != cudaSuccess) rc = fail(FC_E_CUDA, "upload of the prompt failed");
@@ -616,6 +706,11 @@ int prime_window(fc_llama_cache* s, const int32_t* ids, int n) {
                                      s->state, st));
     FC_TRY(check_status(m));
     s->host_pos = n;
+    if (k.on) {
+        k.held = n <= k.cap ? n : k.budget;
+        llama_set_words_kernel<<<1, 1, 0, st>>>(k.words, k.set, k.held, 0);
+        FC_LAUNCHED();
+    }
     return FC_OK;
 }
 
@@ -887,19 +982,33 @@ int fc_llama_score_sequences(fc_llama* m, const int32_t* ids, int n_seq, int seq
 
 float fc_llama_last_score_ms(const fc_llama* m) { return m ? m->last_score_ms : 0.0f; }
 
-int fc_llama_cache_create(fc_llama* m, fc_llama_cache** out) {
-    if (!m || !out) return fail(FC_E_ARG, "fc_llama_cache_create: null argument");
-    *out = nullptr;
+// kv4: the layout of a 4-bit cache (its sizes checked), or null.
+static int cache_create(fc_llama* m, const LlamaKv4* kv4, fc_llama_cache** out) {
     FC_CUDA(cudaSetDevice(m->device));
     const fc_llama_config& c = m->cfg;
     fc_llama_cache* s = new fc_llama_cache();
     s->m = m;
     s->device = m->device;
     auto build = [&]() -> int {
-        const size_t kv = (size_t)c.n_layer * c.ctx * m->kv_dim;
         Arena& a = s->arena;
-        FC_TRY(a.alloc_n(&s->kc, kv));
-        FC_TRY(a.alloc_n(&s->vc, kv));
+        if (kv4) {
+            FC_TRY(scratch_retain(m->device));
+            s->scratch = true;
+            LlamaKv4& k = s->kv4;
+            k = *kv4;
+            const bool evicts = k.cap < c.ctx;
+            for (int i = 0; i < (evicts ? 2 : 1); ++i) {
+                k.layers[i].resize(c.n_layer);
+                for (Kv4& layer : k.layers[i]) FC_TRY(kv4_make(a, 1, c.n_kv_head, c.head_dim, k.cap, &layer));
+                if (evicts) FC_TRY(a.alloc_n(&k.mass[i], (size_t)c.n_layer * c.n_kv_head * k.cap));
+            }
+            FC_TRY(a.alloc_n(&k.words, 4));
+            k.on = true;
+        } else {
+            const size_t kv = (size_t)c.n_layer * c.ctx * m->kv_dim;
+            FC_TRY(a.alloc_n(&s->kc, kv));
+            FC_TRY(a.alloc_n(&s->vc, kv));
+        }
         FC_TRY(a.alloc_n(&s->x, (size_t)c.d_model));
         FC_TRY(a.alloc_n(&s->n, (size_t)c.d_model));
         FC_TRY(a.alloc_n(&s->qkv, (size_t)m->qkv_dim));
@@ -910,8 +1019,9 @@ int fc_llama_cache_create(fc_llama* m, fc_llama_cache** out) {
         s->queue_cap = c.ctx + 1;
         FC_TRY(a.alloc_n(&s->queue, (size_t)s->queue_cap));
         FC_TRY(a.alloc_n(&s->state, 1));
-        FC_TRY(attn_step_split(c.n_head, c.head_dim, c.ctx, &s->attn_split, &s->split_from));
-        if (halves_cover(m)) {
+        if (!kv4) FC_TRY(attn_step_split(c.n_head, c.head_dim, c.ctx, &s->attn_split, &s->split_from));
+        else s->split_from = INT_MAX;
+        if (!kv4 && halves_cover(m)) {
             FC_TRY(a.alloc_n(&s->parts, (size_t)(c.n_head + block_step_slices(c.d_ff, true) + 2) * c.d_model));
             s->split_from = INT_MAX;
         }
@@ -926,6 +1036,29 @@ int fc_llama_cache_create(fc_llama* m, fc_llama_cache** out) {
     return FC_OK;
 }
 
+int fc_llama_cache_create(fc_llama* m, fc_llama_cache** out) {
+    if (!m || !out) return fail(FC_E_ARG, "fc_llama_cache_create: null argument");
+    *out = nullptr;
+    return cache_create(m, nullptr, out);
+}
+
+int fc_llama_cache_create_kv4(fc_llama* m, int capacity, int budget, int recent, fc_llama_cache** out) {
+    if (!m || !out) return fail(FC_E_ARG, "fc_llama_cache_create_kv4: null argument");
+    *out = nullptr;
+    const fc_llama_config& c = m->cfg;
+    if (c.head_dim % kKvBlock) return fail(FC_E_SHAPE, "fc_llama_cache_create_kv4: head_dim %d must be a multiple of %d", c.head_dim, kKvBlock);
+    LlamaKv4 k;
+    k.cap = capacity ? capacity : c.ctx;
+    k.budget = budget;
+    k.recent = recent;
+    if (k.cap < 0 || k.cap > c.ctx) return fail(FC_E_DIM, "fc_llama_cache_create_kv4: capacity %d (0..%d)", capacity, c.ctx);
+    if (k.cap < c.ctx && (budget <= 0 || budget >= k.cap || recent < 0 || recent > budget))
+        return fail(FC_E_SHAPE, "fc_llama_cache_create_kv4: budget %d must be positive and below the capacity %d, recent %d at most the budget", budget, k.cap, recent);
+    return cache_create(m, &k, out);
+}
+
+int fc_llama_cache_held(const fc_llama_cache* s) { return !s ? 0 : s->kv4.on ? s->kv4.held : s->host_pos; }
+
 void fc_llama_cache_free(fc_llama_cache* s) {
     if (!s) return;
     cudaSetDevice(s->device);
@@ -934,6 +1067,7 @@ void fc_llama_cache_free(fc_llama_cache* s) {
     if (s->ev0) cudaEventDestroy(s->ev0);
     if (s->ev1) cudaEventDestroy(s->ev1);
     s->arena.release();
+    if (s->scratch) scratch_release(s->device);
     delete s;
 }
 
@@ -942,6 +1076,11 @@ int fc_llama_cache_clear(fc_llama_cache* s) {
     FC_CUDA(cudaSetDevice(s->m->device));
     llama_set_state_kernel<<<1, 1, 0, s->m->st>>>(s->state, 0, 0, 0);
     FC_LAUNCHED();
+    if (s->kv4.on) {
+        llama_set_words_kernel<<<1, 1, 0, s->m->st>>>(s->kv4.words, s->kv4.set, 0, 0);
+        FC_LAUNCHED();
+        s->kv4.held = 0;
+    }
     s->host_pos = 0;
     return FC_OK;
 }
@@ -1006,11 +1145,12 @@ int fc_llama_generate(fc_llama_cache* s, const int32_t* prompt, int n, int max_n
     while (made < max_new) {
         if (cancel && *cancel) { cancelled = true; break; }
         // all but the last tokens of a free run, once a packed step has run uncaptured
-        if (free_run && max_new - made > kFreeSteps && (m->prec < 0 || s->packed_warm[1])) {
+        if (free_run && max_new - made > kFreeSteps && (m->prec < 0 || s->packed_warm[1]) && (!s->kv4.evicts() || s->kv4.held + kFreeSteps <= s->kv4.cap)) {
             rc = run_graph(s, 2, s->host_pos);
             if (rc != FC_OK) break;
             made += kFreeSteps;
             s->host_pos += kFreeSteps;
+            s->kv4.held += kFreeSteps;
             continue;
         }
         // recent = prompt + tokens so far = the queue (llm.rs:740-751)
@@ -1031,9 +1171,11 @@ int fc_llama_generate(fc_llama_cache* s, const int32_t* prompt, int n, int max_n
         // the forward of the last requested token keeps the cache continuable (llm.rs:750-751); its logits are not used
         // here, so it stays outside the timed region
         if (made == max_new) { FC_CUDA(cudaEventRecord(s->ev1, st)); timed = true; }
-        rc = run_step(s, 1, s->host_pos);                    // forward_one(next), the last token included (llm.rs:750-751)
+        rc = make_room(s, 1);
+        if (rc == FC_OK) rc = run_step(s, 1, s->host_pos);   // forward_one(next), the last token included (llm.rs:750-751)
         if (rc != FC_OK) break;
         s->host_pos += 1;
+        s->kv4.held += 1;
     }
     if (rc == FC_OK) {
         if (!timed) FC_CUDA(cudaEventRecord(s->ev1, st));

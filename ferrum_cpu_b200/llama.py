@@ -22,10 +22,13 @@ def gguf_probe(path):
 class CudaLlamaCache:
     """LlamaCache (llm.rs:522-546): per-layer KV rows and the position of the next token."""
 
-    def __init__(self, model):
+    def __init__(self, model, kv4=False, capacity=0, budget=0, recent=0):
         self.model = model
         self._h = C.c_void_p()
-        check(_lib.lib().fc_llama_cache_create(model._h, C.byref(self._h)))
+        if kv4:
+            check(_lib.lib().fc_llama_cache_create_kv4(model._h, capacity, budget, recent, C.byref(self._h)))
+        else:
+            check(_lib.lib().fc_llama_cache_create(model._h, C.byref(self._h)))
         model._caches.append(weakref.ref(self))
 
     def close(self):
@@ -44,6 +47,10 @@ class CudaLlamaCache:
 
     def pos(self):
         return _lib.lib().fc_llama_cache_pos(self._h)
+
+    def held(self):
+        """Positions the cache holds: pos() less what was evicted."""
+        return _lib.lib().fc_llama_cache_held(self._h)
 
     @property
     def last_decode_ms(self):
@@ -145,8 +152,10 @@ class CudaLlama:
         return _lib.lib().fc_llama_last_score_ms(self._h)
 
     # ---- KV-cached decode ------------------------------------------------------------------
-    def new_cache(self):
-        return CudaLlamaCache(self)
+    def new_cache(self, kv4=False, capacity=0, budget=0, recent=0):
+        """kv4: keys and values in 4-bit levels. With a capacity below the model's context, a cache that has run full keeps its last
+        `recent` positions and the most attended of the others, `budget` in all."""
+        return CudaLlamaCache(self, kv4, capacity, budget, recent)
 
     def forward_one(self, token, cache, want_logits=True):
         """llm.rs:610-618: next-token logits; advances the cache."""

@@ -168,6 +168,8 @@ extern "C" {
     pub fn fc_llama_score_sequences(m: *mut fc_llama, ids: *const i32, n_seq: c_int, seq_len: c_int, batch_windows: c_int, scores: *mut fc_score, lp: *mut f32) -> c_int;
     pub fn fc_llama_last_score_ms(m: *const fc_llama) -> f32;
     pub fn fc_llama_cache_create(m: *mut fc_llama, out: *mut *mut fc_llama_cache) -> c_int;
+    pub fn fc_llama_cache_create_kv4(m: *mut fc_llama, capacity: c_int, budget: c_int, recent: c_int, out: *mut *mut fc_llama_cache) -> c_int;
+    pub fn fc_llama_cache_held(c: *const fc_llama_cache) -> c_int;
     pub fn fc_llama_cache_free(c: *mut fc_llama_cache);
     pub fn fc_llama_cache_clear(c: *mut fc_llama_cache) -> c_int;
     pub fn fc_llama_cache_pos(c: *const fc_llama_cache) -> c_int;

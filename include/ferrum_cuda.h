@@ -459,6 +459,14 @@ int fc_llama_score_sequences(fc_llama* m, const int32_t* ids, int n_seq, int seq
 float fc_llama_last_score_ms(const fc_llama* m);
 
 int fc_llama_cache_create(fc_llama* m, fc_llama_cache** out);
+/* The same cache with its keys and values in 4-bit levels (fc_kv4_create has the format; head_dim a multiple of 32): 1/7 of the
+ * memory. Attention, prompts included, is over what the cache holds. capacity 0: the model's context. With a smaller one, a cache that
+ * has run full keeps the last `recent` positions and those others that have received most attention so far, a key / value
+ * head and layer at a time, `budget` (below the capacity) in all; so does one whose prompt is longer than the capacity. Rotations
+ * and the context window go by the positions of the ids, not by the places that they hold. */
+int fc_llama_cache_create_kv4(fc_llama* m, int capacity, int budget, int recent, fc_llama_cache** out);
+/* Positions that the cache holds: its position, less what was evicted. */
+int fc_llama_cache_held(const fc_llama_cache* c);
 void fc_llama_cache_free(fc_llama_cache* c);
 int fc_llama_cache_clear(fc_llama_cache* c);   /* LlamaCache::clear, llm.rs:536-541 */
 int fc_llama_cache_pos(const fc_llama_cache* c);
