@@ -13,6 +13,8 @@
 // maximum and sum the attention has left; each position is added up by one warp in one order.
 #include <cooperative_groups.h>
 
+#include <climits>
+
 #include "kv4_frag.cuh"
 
 namespace fc {
@@ -25,14 +27,15 @@ constexpr int KT = 64;                           // positions a tile
 
 template <int NB>
 struct PromptShape {
-    static constexpr int WARPS = NB <= 4 ? 8 : 4, COLS = 16 * WARPS, DIM = NB * kKvBlock, PAD = DIM + 4;
+    static constexpr int WARPS = NB <= 4 ? 8 : 4, LAY = WARPS < 8 ? WARPS : 8;          // of which LAY lay the tiles
+    static constexpr int COLS = 16 * WARPS, DIM = NB * kKvBlock, PAD = DIM + 4;
     static constexpr int KBYTES = NB * 4096, VBYTES = NB * 4096;                       // levels as fragments
     static constexpr int KD = KBYTES + VBYTES, VD = KD + NB * KT * 4, EX = VD + NB * KT * 2, BYTES = EX + KT * 8;   // scales; {e, 2^-e}
     static constexpr bool QS = NB > 4;           // q in shared memory
     static constexpr int QBYTES = QS ? COLS * DIM * 4 : 0;
     static constexpr int JOIN = COLS * PAD * 4;
     static constexpr int SMEM = QBYTES + (2 * BYTES > JOIN ? 2 * BYTES : JOIN);
-    static constexpr int CTAS = NB <= 2 ? 2 : 1;
+    static constexpr int CTAS = 1;
 };
 
 __device__ __forceinline__ uint32_t hmul2u(uint32_t a, uint32_t b) {
@@ -159,14 +162,15 @@ template <int NB>
 __global__ void __launch_bounds__(32 * PromptShape<NB>::WARPS, PromptShape<NB>::CTAS)
 kv4_prompt_kernel(Kv4 c, Kv4Attend a, KvRows rows, int cs, float2* __restrict__ stats) {
     using S = PromptShape<NB>;
-    constexpr int WARPS = S::WARPS, DIM = S::DIM, PAD = S::PAD, THREADS = 32 * WARPS, PASS = 8 / WARPS;
+    constexpr int WARPS = S::WARPS, DIM = S::DIM, PAD = S::PAD, THREADS = 32 * WARPS, PASS = 8 / S::LAY;
     extern __shared__ __align__(16) char smem[];
     __shared__ float2 ml[S::COLS];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const int rank = blockIdx.x % cs, h = blockIdx.y, seq = blockIdx.z;
+    const int rank = blockIdx.x % cs, h = blockIdx.x / cs % c.n_kv, seq = blockIdx.z;
     const int first = rows.start[seq], n = rows.start[seq + 1] - first, all_cols = n * a.group;
-    // the last columns see most: they go first
-    const int col0 = (int)(gridDim.x / cs - 1 - blockIdx.x / cs) * S::COLS, cols = min(all_cols - col0, S::COLS);
+    // the last columns, of all heads, see most: they go first
+    const unsigned share = cs * c.n_kv;
+    const int col0 = (int)(gridDim.x / share - 1 - blockIdx.x / share) * S::COLS, cols = min(all_cols - col0, S::COLS);
     if (cols <= 0) return;                       // the whole cluster
     const int len = a.lens[seq], end = a.k ? len + n : len;
     float* const out = a.out + (size_t)first * a.ldo + (size_t)h * a.group * DIM;
@@ -182,7 +186,8 @@ kv4_prompt_kernel(Kv4 c, Kv4Attend a, KvRows rows, int cs, float2* __restrict__ 
     char* const bufs = smem + S::QBYTES;
 
     RawTile<NB, PASS> raw;
-    if (rank < tiles) tile_ask<NB, PASS>(c, row0 + (size_t)rank * KT, tid, raw);
+    const bool lays = tid < 32 * S::LAY;
+    if (lays && rank < tiles) tile_ask<NB, PASS>(c, row0 + (size_t)rank * KT, tid, raw);
 
     const int ca = warp * 16 + g, cb = ca + 8;    // this lane's two columns
     uint32_t qh[NB][8], ql[NB][8];
@@ -212,22 +217,18 @@ kv4_prompt_kernel(Kv4 c, Kv4Attend a, KvRows rows, int cs, float2* __restrict__ 
 
     float o[NB][4][4] = {}, ma = -INFINITY, mb = -INFINITY, la = 0.0f, lb = 0.0f;
     int flip = 0;
-    if (rank < tiles) tile_lay<NB, PASS>(bufs, tid, raw);
+    if (lays && rank < tiles) tile_lay<NB, PASS>(bufs, tid, raw);
     __syncthreads();
     for (int tile = rank; tile < tiles; tile += cs) {
         const char* buf = bufs + flip * S::BYTES;
-        if (tile + cs < tiles) tile_ask<NB, PASS>(c, row0 + (size_t)(tile + cs) * KT, tid, raw);
+        if (lays && tile + cs < tiles) tile_ask<NB, PASS>(c, row0 + (size_t)(tile + cs) * KT, tid, raw);
         const int j0 = tile * KT;
         if (j0 < warp_last) {
             float s[8][4];
             const float* kd = (const float*)(buf + S::KD);
-            constexpr int NG = S::QS ? 4 : 1;     // tiles of 8 positions that share a reading of q
+            constexpr int NG = 4;                 // tiles of 8 positions side by side: four products between two of one sum
 #pragma unroll
             for (int n0 = 0; n0 < 8; n0 += NG) {
-#pragma unroll
-                for (int i = 0; i < NG; ++i)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) s[n0 + i][e] = 0.0f;
 #pragma unroll
                 for (int b = 0; b < NB; ++b) {
                     uint32_t h0[4], h1[4], r0[4], r1[4];
@@ -239,19 +240,23 @@ kv4_prompt_kernel(Kv4 c, Kv4Attend a, KvRows rows, int cs, float2* __restrict__ 
 #pragma unroll
                         for (int e = 0; e < 4; ++e) { h0[e] = qh[b][e]; h1[e] = qh[b][4 + e]; r0[e] = ql[b][e]; r1[e] = ql[b][4 + e]; }
                     }
+                    uint4 f[NG];
+                    float x[NG][4] = {};
+#pragma unroll
+                    for (int i = 0; i < NG; ++i) f[i] = ((const uint4*)buf)[(b * 8 + n0 + i) * 32 + lane];
+#pragma unroll
+                    for (int i = 0; i < NG; ++i) mma16816(x[i], r0, f[i].x, f[i].y);
+#pragma unroll
+                    for (int i = 0; i < NG; ++i) mma16816(x[i], r1, f[i].z, f[i].w);
+#pragma unroll
+                    for (int i = 0; i < NG; ++i) mma16816(x[i], h0, f[i].x, f[i].y);
+#pragma unroll
+                    for (int i = 0; i < NG; ++i) mma16816(x[i], h1, f[i].z, f[i].w);
 #pragma unroll
                     for (int i = 0; i < NG; ++i) {
-                        const uint4 f = ((const uint4*)buf)[(b * 8 + n0 + i) * 32 + lane];
                         const float2 d = *(const float2*)(kd + b * KT + 8 * (n0 + i) + 2 * t);
-                        float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                        mma16816(x, r0, f.x, f.y);
-                        mma16816(x, r1, f.z, f.w);
-                        mma16816(x, h0, f.x, f.y);
-                        mma16816(x, h1, f.z, f.w);
-                        s[n0 + i][0] = fmaf(x[0], d.x, s[n0 + i][0]);
-                        s[n0 + i][1] = fmaf(x[1], d.y, s[n0 + i][1]);
-                        s[n0 + i][2] = fmaf(x[2], d.x, s[n0 + i][2]);
-                        s[n0 + i][3] = fmaf(x[3], d.y, s[n0 + i][3]);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) s[n0 + i][e] = b ? fmaf(x[i][e], e & 1 ? d.y : d.x, s[n0 + i][e]) : x[i][e] * (e & 1 ? d.y : d.x);
                     }
                 }
             }
@@ -337,7 +342,7 @@ kv4_prompt_kernel(Kv4 c, Kv4Attend a, KvRows rows, int cs, float2* __restrict__ 
             }
         }
         flip ^= 1;
-        if (tile + cs < tiles) tile_lay<NB, PASS>(bufs + flip * S::BYTES, tid, raw);
+        if (lays && tile + cs < tiles) tile_lay<NB, PASS>(bufs + flip * S::BYTES, tid, raw);
         __syncthreads();
     }
     la += __shfl_xor_sync(0xffffffffu, la, 1);
@@ -414,10 +419,10 @@ __global__ void __launch_bounds__(32 * WW) kv4_weights_kernel(Kv4 c, Kv4Attend a
     constexpr int DIM = NB * kKvBlock, TILES = S::TILES, BUFS = S::BUFS;
     extern __shared__ __align__(16) char smem[]; // [buffer]: fragments [16 columns][block, plane and fragment][lane], columns
     __shared__ float part[S::POS];
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3, rank = blockIdx.x % cs, h = blockIdx.y, seq = blockIdx.z;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3, rank = blockIdx.x % cs, h = blockIdx.x / cs % c.n_kv, seq = blockIdx.z;
     const int first = rows.start[seq], n = rows.start[seq + 1] - first, all_cols = n * a.group;
     const int len = a.lens[seq], end = a.k ? len + n : len;
-    const int j00 = blockIdx.x / cs * S::POS, j0 = j00 + warp * (8 * TILES), base = end - n + 1;
+    const int j00 = blockIdx.x / (cs * c.n_kv) * S::POS, j0 = j00 + warp * (8 * TILES), base = end - n + 1;
     if (n == 0 || len < 0 || len > c.cap - (a.k ? n : 0) || j00 >= end) return;      // the whole cluster
     // levels and scales of the warp's positions
     uint32_t kf[TILES][NB][4];
@@ -544,11 +549,12 @@ int launch_prompt_t(const Kv4& c, const Kv4Attend& a, const KvRows& rows, int ma
         if (device < 64) attr_set[device] = true;
     }
     const long long tiles = ((long long)max_rows * a.group + S::COLS - 1) / S::COLS, ctas = tiles * c.n_kv * c.n_seq;
+    if (tiles * 8 * c.n_kv > INT_MAX) return fail(FC_E_SHAPE, "%d rows of %d heads are too many for one call", max_rows, c.n_kv * a.group);
     // a cluster shares the positions where there are fewer CTAs than the GPU holds, two tiles each at least
     int cs = 1;
     while (cs < 8 && ctas * cs * 2 <= 148 * S::CTAS && cs * 4 * KT <= c.cap) cs *= 2;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(tiles * cs), c.n_kv, c.n_seq);
+    cfg.gridDim = dim3((unsigned)(tiles * cs * c.n_kv), 1, c.n_seq);
     cfg.blockDim = dim3(32 * S::WARPS);
     cfg.dynamicSmemBytes = S::SMEM;
     cfg.stream = st;
@@ -575,7 +581,7 @@ int launch_weights_t(const Kv4& c, const Kv4Attend& a, const KvRows& rows, int m
     int cs = 1;
     while (cs < 8 && cs * 4 <= passes && ctas * cs < 148 * 8) cs *= 2;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(tiles * cs), c.n_kv, c.n_seq);
+    cfg.gridDim = dim3((unsigned)(tiles * cs * c.n_kv), 1, c.n_seq);
     cfg.blockDim = dim3(32 * WW);
     cfg.dynamicSmemBytes = S::SMEM;
     cfg.stream = st;
