@@ -21,10 +21,10 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int COLS = 8, TILE = 32;                // columns of a product, positions a tile
+constexpr int SW = 8, COLS = 8, TILE = 32;        // warps, columns of a product, positions a tile
 constexpr int kStepRows = 32;                     // most new rows of a sequence
 
-template <int NB, int SW>
+template <int NB>
 struct StepShape {
     static constexpr int DIM = NB * kKvBlock, PAD = DIM + 4;
     static constexpr int STAGES = NB <= 2 ? 3 : 2;
@@ -32,12 +32,12 @@ struct StepShape {
     static constexpr int RING = SW * STAGES * BYTES;
     static constexpr int FRESH = kStepRows * NB * 36;    // new rows, quantised; then the CTA's joined result
     static constexpr int SMEM = RING + (FRESH > COLS * PAD * 4 ? FRESH : COLS * PAD * 4);
-    static constexpr int CTAS = (NB <= 4 ? 16 : 8) / SW;
+    static constexpr int CTAS = NB <= 4 ? 2 : 1;
 };
 
 template <int NB>
 __device__ __forceinline__ void ask(const Kv4& c, size_t row, char* tile, int lane, bool values) {
-    using S = StepShape<NB, 8>;
+    using S = StepShape<NB>;
     const char *kq = (const char*)(c.kq + row * (NB * 4)), *vq = (const char*)(c.vq + row * (NB * 4));
 #pragma unroll
     for (int i = 0; i < NB; ++i) cp16(tile + i * 512 + lane * 16, kq + i * 512 + lane * 16);
@@ -62,7 +62,7 @@ struct Query {
 // columns 2 t and + 1, s[m][2..3] position 16 m + g + 8. With `edge`, -inf behind what a column sees.
 template <int NB, bool SPLIT>
 __device__ __forceinline__ void tile_scores(const char* tile, const Query<NB, SPLIT>& q, bool edge, int j0, int seen0, int seen1, int g, int t, float (&s)[2][SPLIT ? 2 : 4]) {
-    using S = StepShape<NB, 8>;
+    using S = StepShape<NB>;
     const uint32_t* kq = (const uint32_t*)tile;
     const __half* kd = (const __half*)(tile + 2 * S::KBYTES);
 #pragma unroll
@@ -130,9 +130,9 @@ __device__ __forceinline__ uint32_t hmax2u(uint32_t a, uint32_t b) {
     return *(const uint32_t*)&r;
 }
 
-template <int NB, bool SPLIT, int SW>
-__global__ void __launch_bounds__(32 * SW, StepShape<NB, SW>::CTAS) kv4_step_kernel(Kv4 c, Kv4Attend a, KvRows rows, float2* __restrict__ stats) {
-    using S = StepShape<NB, SW>;
+template <int NB, bool SPLIT>
+__global__ void __launch_bounds__(32 * SW, StepShape<NB>::CTAS) kv4_step_kernel(Kv4 c, Kv4Attend a, KvRows rows, float2* __restrict__ stats) {
+    using S = StepShape<NB>;
     constexpr int DIM = S::DIM, PAD = S::PAD, CALL = SPLIT ? COLS / 2 : COLS;      // columns of a call
     extern __shared__ __align__(16) char smem[];
     __shared__ float2 warp_ml[SW][COLS];          // running maximum (base 2) and sum
@@ -483,8 +483,29 @@ __global__ void __launch_bounds__(32 * SW, StepShape<NB, SW>::CTAS) kv4_step_ker
             if (last - i * stride >= 0) ask<NB>(c, row0 + (size_t)(last - i * stride) * TILE, ring + i * S::BYTES, lane, false);
             cp_commit();
         }
+        // what the tile's positions had is asked for a tile ahead
+        constexpr int EACH = SPLIT ? 1 : 2;
+        const bool mine_to_add = (SPLIT ? t & 1 : t) == 0;
+        const int old_end = a.k ? len : end;
+        auto spot = [&](int tile, int m, int u) { return tile * TILE + 16 * m + g + 8 * (SPLIT ? t >> 1 : u); };
+        float had[2][EACH], next[2][EACH] = {};
+        auto ask_mass = [&](int tile, float (&x)[2][EACH]) {
+#pragma unroll
+            for (int m = 0; m < 2; ++m)
+#pragma unroll
+                for (int u = 0; u < EACH; ++u) {
+                    const int j = spot(tile, m, u);
+                    x[m][u] = mine_to_add && tile >= 0 && j < old_end ? mass[j] : 0.0f;
+                }
+        };
+        ask_mass(last, next);
         stage = 0;
         for (int tile = last; tile >= 0; tile -= stride) {
+#pragma unroll
+            for (int m = 0; m < 2; ++m)
+#pragma unroll
+                for (int u = 0; u < EACH; ++u) had[m][u] = next[m][u];
+            ask_mass(tile - stride, next);
             if (tile != last) {
                 cp_wait<S::STAGES - 2>();
                 __syncwarp();
@@ -497,12 +518,12 @@ __global__ void __launch_bounds__(32 * SW, StepShape<NB, SW>::CTAS) kv4_step_ker
 #pragma unroll
             for (int m = 0; m < 2; ++m)
 #pragma unroll
-                for (int u = 0; u < (SPLIT ? 1 : 2); ++u) {
+                for (int u = 0; u < EACH; ++u) {
                     float x = (l0 != 0.0f ? ex2(s[m][2 * u] - z0) * l0 : 0.0f) + (l1 != 0.0f ? ex2(s[m][2 * u + 1] - z1) * l1 : 0.0f);
                     x += __shfl_xor_sync(0xffffffffu, x, 1);
                     if (!SPLIT) x += __shfl_xor_sync(0xffffffffu, x, 2);
-                    const int j = tile * TILE + 16 * m + g + 8 * (SPLIT ? t >> 1 : u);
-                    if ((SPLIT ? t & 1 : t) == 0 && j < end) mass[j] = (j < (a.k ? len : end) ? mass[j] : 0.0f) + x;
+                    const int j = spot(tile, m, u);
+                    if (mine_to_add && j < end) mass[j] = had[m][u] + x;
                 }
         }
         return;
@@ -510,10 +531,10 @@ __global__ void __launch_bounds__(32 * SW, StepShape<NB, SW>::CTAS) kv4_step_ker
     if (cs > 1) cluster.sync();                   // no rank leaves while another reads its memory
 }
 
-template <int NB, bool SPLIT, int SW>
+template <int NB, bool SPLIT>
 int launch_step_t(const Kv4& c, const Kv4Attend& a, const KvRows& rows, int groups, float2* stats, int device, cudaStream_t st) {
-    using S = StepShape<NB, SW>;
-    const auto kernel = kv4_step_kernel<NB, SPLIT, SW>;
+    using S = StepShape<NB>;
+    const auto kernel = kv4_step_kernel<NB, SPLIT>;
     static bool attr_set[64] = {};
     if (device >= 64 || !attr_set[device]) {
         FC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM));
@@ -544,9 +565,7 @@ template <int NB>
 int launch_step_nb(const Kv4& c, const Kv4Attend& a, const KvRows& rows, int cols, float2* stats, int device, cudaStream_t st) {
     const bool split = cols <= COLS / 2;
     const int groups = split ? 1 : (cols + COLS - 1) / COLS;
-    const bool many = (long long)c.n_seq * c.n_kv * groups > 148;
-    if (split) return many ? launch_step_t<NB, true, 4>(c, a, rows, groups, stats, device, st) : launch_step_t<NB, true, 8>(c, a, rows, groups, stats, device, st);
-    return many ? launch_step_t<NB, false, 4>(c, a, rows, groups, stats, device, st) : launch_step_t<NB, false, 8>(c, a, rows, groups, stats, device, st);
+    return split ? launch_step_t<NB, true>(c, a, rows, groups, stats, device, st) : launch_step_t<NB, false>(c, a, rows, groups, stats, device, st);
 }
 
 }  // namespace
