@@ -88,7 +88,7 @@ __device__ __forceinline__ unsigned weight_key(float w) {
     return w != w ? 0u : b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u);
 }
 
-constexpr int ET = 512, BINS = 2048, KEYS = 16384, LISTED = 2048;
+constexpr int ET = 1024, BINS = 2048, KEYS = 16384, LISTED = 2048;
 struct __align__(16) EvictShared {
     unsigned key[KEYS];
     unsigned bins[BINS];
@@ -100,7 +100,7 @@ struct __align__(16) EvictShared {
 // What stays of a (sequence, head), shared by gridDim.x CTAs. Each finds the key of the last position that stays for itself (three passes
 // of 11, 11 and 10 bits over the keys, in shared memory where they fit): the row of weights is short next to what is moved, and no CTA has to
 // wait for another. Then each brings a range of dst's rows. Bound: latency, and the bytes moved of long caches.
-__global__ void __launch_bounds__(ET, 2) kv4_evict_kernel(Kv4 src, Kv4 dst, const int* __restrict__ lens, int* __restrict__ lens_out, int budget, int recent,
+__global__ void __launch_bounds__(ET, 1) kv4_evict_kernel(Kv4 src, Kv4 dst, const int* __restrict__ lens, int* __restrict__ lens_out, int budget, int recent,
                                                           const float* __restrict__ mass, float* __restrict__ mass_out, int* __restrict__ kept) {
     extern __shared__ __align__(16) char raw[];
     EvictShared& s = *(EvictShared*)raw;
@@ -157,10 +157,11 @@ __global__ void __launch_bounds__(ET, 2) kv4_evict_kernel(Kv4 src, Kv4 dst, cons
                 }
             }
             __syncthreads();
-            // from the largest digit down: four a thread
-            int n[4], sum = 0;
+            // from the largest digit down: EACH a thread
+            constexpr int EACH = BINS / ET;
+            int n[EACH], sum = 0;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) { n[i] = (int)s.bins[BINS - 1 - (4 * tid + i)]; sum += n[i]; }
+            for (int i = 0; i < EACH; ++i) { n[i] = (int)s.bins[BINS - 1 - (EACH * tid + i)]; sum += n[i]; }
             int incl = sum;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -172,9 +173,9 @@ __global__ void __launch_bounds__(ET, 2) kv4_evict_kernel(Kv4 src, Kv4 dst, cons
             int before = incl - sum;
             for (int w = 0; w < warp; ++w) before += s.warp_n[w];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
+            for (int i = 0; i < EACH; ++i) {
                 if (before < ties && before + n[i] >= ties) {
-                    s.digit = BINS - 1 - (4 * tid + i);
+                    s.digit = BINS - 1 - (EACH * tid + i);
                     s.above = before;
                     if (pass == 0) s.in_bin = n[i];
                 }
@@ -276,16 +277,12 @@ int launch_kv4_append(const Kv4& c, const float* k, const float* v, int ldkv, co
 int kv4_make(Arena& arena, int n_seq, int n_kv, int dim, int cap, Kv4* c) {
     const int pad = (cap + kKvTile - 1) / kKvTile * kKvTile;
     const size_t rows = (size_t)n_seq * n_kv * pad, q = rows * dim / 2, d = rows * (dim / kKvBlock) * 2;
-    *c = Kv4{nullptr, nullptr, nullptr, nullptr, n_seq, n_kv, dim / kKvBlock, cap, pad};
-    FC_TRY(arena.alloc((void**)&c->kq, q));
-    FC_TRY(arena.alloc((void**)&c->vq, q));
-    FC_TRY(arena.alloc((void**)&c->kd, d));
-    FC_TRY(arena.alloc((void**)&c->vd, d));
-    FC_CUDA(cudaMemset(c->kq, 0, q));
-    FC_CUDA(cudaMemset(c->vq, 0, q));
-    FC_CUDA(cudaMemset(c->kd, 0, d));
-    FC_CUDA(cudaMemset(c->vd, 0, d));
-    FC_CUDA(cudaDeviceSynchronize());
+    // one allocation: rows are padded to 64, so that each part is a multiple of 128 bytes
+    char* p = nullptr;
+    FC_TRY(arena.alloc((void**)&p, 2 * (q + d)));
+    FC_CUDA(cudaMemset(p, 0, 2 * (q + d)));
+    FC_CUDA(cudaStreamSynchronize(0));
+    *c = Kv4{(uint32_t*)p, (uint32_t*)(p + q), (__half*)(p + 2 * q), (__half*)(p + 2 * q + d), n_seq, n_kv, dim / kKvBlock, cap, pad};
     return FC_OK;
 }
 
@@ -296,10 +293,11 @@ int launch_kv4_evict(const Kv4& a, const Kv4& b, const int* lens, int* lens_out,
         FC_CUDA(cudaFuncSetAttribute(kv4_evict_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(EvictShared)));
         if (device < 64) attr_set[device] = true;
     }
-    // CTAs that share a head: as many as are resident, 64 rows of dst each at least
+    // CTAs that share a head: one an SM, as each looks for the cut (512 threads and two an SM: 33.3 us for 64 heads of 16001, so 26.9); 64
+    // rows of dst each at least
     const long long heads = (long long)a.n_kv * a.n_seq;
     int share = 1;
-    while (share < 32 && heads * share * 2 <= 296 && budget >= share * 2 * 64) share *= 2;
+    while (share < 32 && heads * share * 2 <= 148 && budget >= share * 2 * 64) share *= 2;
     kv4_evict_kernel<<<dim3(share, a.n_kv, a.n_seq), ET, sizeof(EvictShared), st>>>(a, b, lens, lens_out, budget, recent, mass, mass_out, kept);
     FC_LAUNCHED();
     return FC_OK;

@@ -506,11 +506,19 @@ __global__ void __launch_bounds__(32 * WW) kv4_weights_kernel(Kv4 c, Kv4Attend a
                     s[i][3] = fmaf(x[3], kd[i][b].y, s[i][3]);
                 }
             }
+            if (__all_sync(0xffffffffu, min(seen_a, seen_b) >= j0 + 8 * TILES)) {
 #pragma unroll
-            for (int i = 0; i < TILES; ++i) {
-                const int j = j0 + 8 * i + 2 * t;
-                sum[i][0] += (j < seen_a ? ex2(fmaf(s[i][0], xa.x, -xa.y)) * xa.z : 0.0f) + (j < seen_b ? ex2(fmaf(s[i][2], xb.x, -xb.y)) * xb.z : 0.0f);
-                sum[i][1] += (j + 1 < seen_a ? ex2(fmaf(s[i][1], xa.x, -xa.y)) * xa.z : 0.0f) + (j + 1 < seen_b ? ex2(fmaf(s[i][3], xb.x, -xb.y)) * xb.z : 0.0f);
+                for (int i = 0; i < TILES; ++i) {
+                    sum[i][0] = fmaf(ex2(fmaf(s[i][0], xa.x, -xa.y)), xa.z, fmaf(ex2(fmaf(s[i][2], xb.x, -xb.y)), xb.z, sum[i][0]));
+                    sum[i][1] = fmaf(ex2(fmaf(s[i][1], xa.x, -xa.y)), xa.z, fmaf(ex2(fmaf(s[i][3], xb.x, -xb.y)), xb.z, sum[i][1]));
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < TILES; ++i) {
+                    const int j = j0 + 8 * i + 2 * t;
+                    sum[i][0] += (j < seen_a ? ex2(fmaf(s[i][0], xa.x, -xa.y)) * xa.z : 0.0f) + (j < seen_b ? ex2(fmaf(s[i][2], xb.x, -xb.y)) * xb.z : 0.0f);
+                    sum[i][1] += (j + 1 < seen_a ? ex2(fmaf(s[i][1], xa.x, -xa.y)) * xa.z : 0.0f) + (j + 1 < seen_b ? ex2(fmaf(s[i][3], xb.x, -xb.y)) * xb.z : 0.0f);
+                }
             }
         }
         if (BUFS == 2) flip ^= 1;

@@ -497,6 +497,51 @@ def test_a_captured_call_reads_the_lengths_anew(rows):
         assert np.array_equal(a, b)
 
 
+@pytest.mark.gpu
+def test_the_most_sequences_and_few_with_rows():
+    rng = np.random.default_rng(13)
+    run = Run(256, 1, 32, 40)
+    lens = [int(v) for v in rng.integers(0, 38, 256)]
+    fill(run, rng, lens)
+    rows = [0] * 256
+    for s in (0, 3, 77, 200, 255):
+        rows[s] = 2
+    got, q, _ = attend(run, rng, 3, lens, rows)
+    check_attention(run, 3, lens, rows, got, q)
+    got, q, _ = attend(run, rng, 2, lens, [1] * 256)
+    check_attention(run, 2, lens, [1] * 256, got, q)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 3])
+def test_positions_past_32_bits(rows):
+    """Eight heads of 2^24 positions of 256: words and halves lie past 2^32. The rows at the end see nothing but zeros, whose scores are 0:
+    the weight of a new row with score s is e^s / (2^24 - rows + sums of e^s)."""
+    cap, kv, dim = 1 << 24, 8, 256
+    c = kv4.Kv4Cache(1, kv, dim, cap)
+    x = np.zeros((rows, 3 * kv * dim), np.float32)
+    level = np.where(np.arange(dim) % 32 == 0, 1.0, 0.5).astype(np.float32)         # exact in 4 bits: 8 and 4 eighths
+    x[:, :kv * dim] = 17.0 / 16 / np.tile(level, kv) / (dim / 256)                  # q k / 16 = 17
+    x[:, kv * dim:2 * kv * dim] = -np.tile(level, kv)
+    x[:, :kv * dim] *= -1
+    x[:, 2 * kv * dim:] = -np.tile(level, kv) * np.repeat(np.arange(1, kv + 1), dim)
+    xd, lens, out = dev(x), ints([cap - rows]), torch.empty((rows, kv * dim), device="cuda")
+    c.attend_dev(xd.data_ptr(), 3 * kv * dim, kv, lens.data_ptr(), out.data_ptr(), kv * dim, k_ptr=xd.data_ptr() + 4 * kv * dim, v_ptr=xd.data_ptr() + 8 * kv * dim,
+                 ldkv=3 * kv * dim, rows=[rows])
+    got = out.cpu().numpy().astype(np.float64)
+    for i in range(rows):
+        w = (i + 1) * math.exp(17.0) / (cap - rows + (i + 1) * math.exp(17.0))
+        want = w * x[i, 2 * kv * dim:]
+        # a score of 17 in f32: 17 * 264 roundings at the most
+        assert np.abs(got[i] - want).max() <= np.abs(want).max() * (17 * 264 * 2 * EPS + 2.0 ** -18)
+    k, v = (torch.empty((1, 4, kv, dim), device="cuda") for _ in range(2))
+    start = ints([cap - 4])
+    c.read_dev(4, k.data_ptr(), v.data_ptr(), from_ptr=start.data_ptr())
+    for t, at in ((k, kv * dim), (v, 2 * kv * dim)):
+        assert np.array_equal(t[0, 4 - rows:].cpu().numpy().reshape(rows, -1), x[:, at:at + kv * dim]) and not t[0, :4 - rows].any()
+    c.close()
+
+
 # ---- eviction ------------------------------------------------------------------------------------------------------
 def plain_kept(mass, length, budget, recent):
     if length <= budget:

@@ -144,6 +144,24 @@ def test_ties_at_a_cut_all_stay(V):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("V,n", [(9000, 3), (70000, 2), (70000, 300), (300001, 1), (1 << 20, 1), (1 << 20, 5)])
+def test_cuts_among_more_ties_than_are_listed(V, n):
+    """Logits in few steps: thousands of ids share the value at which a cut falls. And rows up to the longest."""
+    rng = np.random.default_rng(V + n)
+    rows = (np.round(2.0 * rng.standard_normal((min(n, 4), V))) / 2).astype(np.float32)
+    rows = rows[np.arange(n) % len(rows)]
+    u = rng.random(n).astype(np.float32)
+    for params in ((1.0, 0, 0.9, 0.0), (0.7, 2000, 1.0, 0.0), (1.2, V // 2, 0.5, 0.0), (1.0, 0, 1.0, 0.01), (1.0, 0, 1 - 2.0 ** -20, 0.0)):
+        token, prob = draw(rows, [params] * n, u)
+        for i in range(min(n, 5)):
+            want, p, near = plain_draw(rows[i], *params, u[i])
+            assert near <= 1e-9 or (token[i] == want and abs(prob[i] - p) <= 2.0 ** -23 * p + 1e-12), (params, i)
+    same = np.zeros((n, V), np.float32)
+    token, prob = draw(same, [(1.0, 5, 0.5, 0.0)] * n, u)            # all tie: all stay
+    assert (np.abs(prob - 1 / V) <= 2.0 ** -23 / V).all() and all(token[i] == plain_draw(same[i], 1.0, 5, 0.5, 0.0, u[i])[0] for i in range(min(n, 3)))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("V", [50, 1000, 131072])
 def test_every_id_is_drawn_as_often_as_its_weight_says(V):
     """u at the middle of each of 4096 even steps: an id's count is 4096 times its probability, to a step at either end."""
