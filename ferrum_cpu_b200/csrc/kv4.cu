@@ -12,6 +12,8 @@ namespace {
 // Rows of k and v into the cache: a warp takes up to four blocks of one row and head, eight lanes a block. Bound: the bytes of long
 // prompts, latency of short ones.
 __global__ void __launch_bounds__(256) kv4_append_kernel(Kv4 c, const float* __restrict__ k, const float* __restrict__ v, int ldkv, KvRows rows, const int* __restrict__ lens) {
+    pdl_trigger();
+    pdl_wait();
     const int lane = threadIdx.x & 31, seq = blockIdx.z, h = blockIdx.y, first = rows.start[seq], n = rows.start[seq + 1] - first;
     const int len = lens[seq];
     if (len < 0 || len > c.cap - n) return;
@@ -41,6 +43,8 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(Kv4 c, const float* __r
 // Positions from[seq] .. + n of every sequence as the values that they stand for: out [n_seq][n][n_kv][dim], zeros outside the cache. A thread
 // writes eight channels of a row, of keys from one word, of values from the nibble j of eight half words. Bound: the bytes written.
 __global__ void __launch_bounds__(256) kv4_read_kernel(Kv4 c, const int* __restrict__ from, int n, float* __restrict__ k, float* __restrict__ v) {
+    pdl_trigger();
+    pdl_wait();
     const int parts = c.nb * 4, seq = blockIdx.y, base = from ? from[seq] : 0;
     const int per = 128 / parts, e = threadIdx.x & 127, part = e % parts, b = part >> 2, t = part & 3;      // rows a block: half of it keys, half values
     const bool values = threadIdx.x >= 128;
@@ -104,6 +108,8 @@ __global__ void __launch_bounds__(ET, 1) kv4_evict_kernel(Kv4 src, Kv4 dst, cons
                                                           const float* __restrict__ mass, float* __restrict__ mass_out, int* __restrict__ kept) {
     extern __shared__ __align__(16) char raw[];
     EvictShared& s = *(EvictShared*)raw;
+    pdl_trigger();
+    pdl_wait();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, h = blockIdx.y, seq = blockIdx.z, head = seq * src.n_kv + h;
     int len = lens[seq];
     len = len < 0 ? 0 : min(len, src.cap);
@@ -269,7 +275,7 @@ __global__ void __launch_bounds__(ET, 1) kv4_evict_kernel(Kv4 src, Kv4 dst, cons
 int launch_kv4_append(const Kv4& c, const float* k, const float* v, int ldkv, const KvRows& rows, int max_rows, const int* lens, cudaStream_t st) {
     const long long warps = (long long)max_rows * ((c.nb + 3) / 4);
     const dim3 grid((unsigned)std::min<long long>((warps + 7) / 8, 4096), c.n_kv, c.n_seq);
-    kv4_append_kernel<<<grid, 256, 0, st>>>(c, k, v, ldkv, rows, lens);
+    FC_CUDA(launch_pdl(kv4_append_kernel, grid, dim3(256), 0, st, c, k, v, ldkv, rows, lens));
     FC_LAUNCHED();
     return FC_OK;
 }
@@ -298,7 +304,7 @@ int launch_kv4_evict(const Kv4& a, const Kv4& b, const int* lens, int* lens_out,
     const long long heads = (long long)a.n_kv * a.n_seq;
     int share = 1;
     while (share < 32 && heads * share * 2 <= 148 && budget >= share * 2 * 64) share *= 2;
-    kv4_evict_kernel<<<dim3(share, a.n_kv, a.n_seq), ET, sizeof(EvictShared), st>>>(a, b, lens, lens_out, budget, recent, mass, mass_out, kept);
+    FC_CUDA(launch_pdl(kv4_evict_kernel, dim3(share, a.n_kv, a.n_seq), dim3(ET), sizeof(EvictShared), st, a, b, lens, lens_out, budget, recent, mass, mass_out, kept));
     FC_LAUNCHED();
     return FC_OK;
 }
@@ -401,7 +407,7 @@ int fc_kv4_read_dev(const fc_kv4* c, const int32_t* from, int n, float* k, float
     if (!aligned16(k) || !aligned16(v)) return fail(FC_E_ARG, "fc_kv4_read_dev: k and v must be 16-byte aligned");
     const int per = 128 / (c->c.nb * 4);
     const dim3 grid((unsigned)std::min<long long>(((long long)n * c->c.n_kv + per - 1) / per, std::max(1, 148 * 16 / c->c.n_seq)), c->c.n_seq);
-    kv4_read_kernel<<<grid, 256, 0, (cudaStream_t)stream>>>(c->c, from, n, k, v);
+    FC_CUDA(launch_pdl(kv4_read_kernel, grid, dim3(256), 0, (cudaStream_t)stream, c->c, from, n, k, v));
     FC_LAUNCHED();
     return FC_OK;
 }

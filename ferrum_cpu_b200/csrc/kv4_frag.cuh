@@ -1,6 +1,7 @@
 // What the attention kernels on the 4-bit cache share: levels as matrix fragments, planes of f32 values, rows into the cache.
 #pragma once
 #include "kv4_ops.cuh"
+#include "pdl.cuh"
 
 namespace fc {
 

@@ -165,6 +165,8 @@ kv4_prompt_kernel(Kv4 c, Kv4Attend a, KvRows rows, int cs, float2* __restrict__ 
     constexpr int WARPS = S::WARPS, DIM = S::DIM, PAD = S::PAD, THREADS = 32 * WARPS, PASS = 8 / S::LAY;
     extern __shared__ __align__(16) char smem[];
     __shared__ float2 ml[S::COLS];
+    pdl_trigger();
+    pdl_wait();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int rank = blockIdx.x % cs, h = blockIdx.x / cs % c.n_kv, seq = blockIdx.z;
     const int first = rows.start[seq], n = rows.start[seq + 1] - first, all_cols = n * a.group;
@@ -419,6 +421,8 @@ __global__ void __launch_bounds__(32 * WW) kv4_weights_kernel(Kv4 c, Kv4Attend a
     constexpr int DIM = NB * kKvBlock, TILES = S::TILES, BUFS = S::BUFS;
     extern __shared__ __align__(16) char smem[]; // [buffer]: fragments [16 columns][block, plane and fragment][lane], columns
     __shared__ float part[S::POS];
+    pdl_trigger();
+    pdl_wait();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3, rank = blockIdx.x % cs, h = blockIdx.x / cs % c.n_kv, seq = blockIdx.z;
     const int first = rows.start[seq], n = rows.start[seq + 1] - first, all_cols = n * a.group;
     const int len = a.lens[seq], end = a.k ? len + n : len;
@@ -561,18 +565,7 @@ int launch_prompt_t(const Kv4& c, const Kv4Attend& a, const KvRows& rows, int ma
     // a cluster shares the positions where there are fewer CTAs than the GPU holds, two tiles each at least
     int cs = 1;
     while (cs < 8 && ctas * cs * 2 <= 148 * S::CTAS && cs * 4 * KT <= c.cap) cs *= 2;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(tiles * cs * c.n_kv), 1, c.n_seq);
-    cfg.blockDim = dim3(32 * S::WARPS);
-    cfg.dynamicSmemBytes = S::SMEM;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = cs;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    FC_CUDA(cudaLaunchKernelEx(&cfg, kv4_prompt_kernel<NB>, c, a, rows, cs, stats));
+    FC_CUDA(launch_pdl_cluster(kv4_prompt_kernel<NB>, dim3((unsigned)(tiles * cs * c.n_kv), 1, c.n_seq), dim3(32 * S::WARPS), S::SMEM, cs, st, c, a, rows, cs, stats));
     FC_LAUNCHED();
     return FC_OK;
 }
@@ -588,18 +581,7 @@ int launch_weights_t(const Kv4& c, const Kv4Attend& a, const KvRows& rows, int m
     // the first positions are seen by all columns, the last by few: a cluster shares the columns, several rounds of CTAs even out the rest
     int cs = 1;
     while (cs < 8 && cs * 4 <= passes && ctas * cs < 148 * 8) cs *= 2;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(tiles * cs * c.n_kv), 1, c.n_seq);
-    cfg.blockDim = dim3(32 * WW);
-    cfg.dynamicSmemBytes = S::SMEM;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = cs;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    FC_CUDA(cudaLaunchKernelEx(&cfg, kv4_weights_kernel<NB>, c, a, rows, cs, stats));
+    FC_CUDA(launch_pdl_cluster(kv4_weights_kernel<NB>, dim3((unsigned)(tiles * cs * c.n_kv), 1, c.n_seq), dim3(32 * WW), S::SMEM, cs, st, c, a, rows, cs, stats));
     FC_LAUNCHED();
     return FC_OK;
 }

@@ -138,6 +138,8 @@ __global__ void __launch_bounds__(32 * SW, StepShape<NB>::CTAS) kv4_step_kernel(
     __shared__ float2 warp_ml[SW][COLS];          // running maximum (base 2) and sum
     __shared__ float warp_f[SW][COLS];
     __shared__ float2 cta_ml[COLS];
+    pdl_trigger();
+    pdl_wait();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int cs = gridDim.x, rank = blockIdx.x, h = blockIdx.y % c.n_kv, col0 = blockIdx.y / c.n_kv * CALL, seq = blockIdx.z;
     const int first = rows.start[seq], n = rows.start[seq + 1] - first, cols = min(n * a.group - col0, CALL);
@@ -545,18 +547,7 @@ int launch_step_t(const Kv4& c, const Kv4Attend& a, const KvRows& rows, int grou
     const int most = (c.cap + TILE * SW - 1) / (TILE * SW);
     int cs = 1;
     while (cs < 8 && cs * 2 <= most && clusters * cs * 2 <= 148 * S::CTAS) cs *= 2;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(cs, c.n_kv * groups, c.n_seq);
-    cfg.blockDim = dim3(32 * SW);
-    cfg.dynamicSmemBytes = S::SMEM;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = cs;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    FC_CUDA(cudaLaunchKernelEx(&cfg, kernel, c, a, rows, stats));
+    FC_CUDA(launch_pdl_cluster(kernel, dim3(cs, c.n_kv * groups, c.n_seq), dim3(32 * SW), S::SMEM, cs, st, c, a, rows, stats));
     FC_LAUNCHED();
     return FC_OK;
 }

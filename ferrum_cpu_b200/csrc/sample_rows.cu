@@ -15,7 +15,7 @@
 // Bound: the instructions of the passes (a weight is 9 operations in f64 and some thirty in all), and for few rows their latency.
 #include <cooperative_groups.h>
 
-#include "fc_common.cuh"
+#include "pdl.cuh"
 
 namespace fc {
 
@@ -180,6 +180,7 @@ __global__ void __launch_bounds__(RT, 4) sample_rows_kernel(const float* __restr
     extern __shared__ __align__(16) char smem_raw[];
     Shared& s = *(Shared*)smem_raw;
     cg::cluster_group cluster = cg::this_cluster();
+    pdl_wait();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, rank = blockIdx.x % cs, r = blockIdx.x / cs;
     const fc_row_sampling p = params[r];
     const float* const in = logits + (size_t)r * ld;
@@ -561,6 +562,8 @@ __global__ void __launch_bounds__(RT, 4) sample_rows_kernel(const float* __restr
         }
         __syncthreads();                      // the warps' sums of the pass have been read
     }
+    // (earlier, the next draw's CTAs would take their places among this one's: 192 rows of 131072 in 199 us, so 174)
+    pdl_trigger();
     if (lane == 0) s.warp_w[warp] = warp_all;
     __syncthreads();
     if (tid == 0) {
@@ -657,18 +660,8 @@ extern "C" int fc_sample_rows_dev(int device, const float* logits, int64_t ld, i
     while ((vocab + cs - 1) / cs > chunk * (CHUNKS - 1)) chunk *= 2;
     const int share = ((vocab + cs - 1) / cs + chunk - 1) / chunk * chunk;
     const bool in_shared = share <= kSlice && (share <= kSlice / 8 || (long long)n_rows * cs <= 148);
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)n_rows * cs);
-    cfg.blockDim = dim3(RT);
-    cfg.dynamicSmemBytes = sizeof(Shared) + (in_shared ? (size_t)share * sizeof(float) : 0);
-    cfg.stream = (cudaStream_t)stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = cs;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    FC_CUDA(cudaLaunchKernelEx(&cfg, sample_rows_kernel, logits, (long long)ld, vocab, params, u, token, prob, cs, chunk, (int)in_shared));
+    FC_CUDA(launch_pdl_cluster(sample_rows_kernel, dim3((unsigned)n_rows * cs), dim3(RT), sizeof(Shared) + (in_shared ? (size_t)share * sizeof(float) : 0), cs, (cudaStream_t)stream,
+                               logits, (long long)ld, vocab, params, u, token, prob, cs, chunk, (int)in_shared));
     FC_LAUNCHED();
     return FC_OK;
 }
