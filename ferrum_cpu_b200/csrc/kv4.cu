@@ -9,40 +9,41 @@ namespace fc {
 
 namespace {
 
-// Rows of k and v into the cache: a warp takes up to four blocks of one row and head, of keys or of values, eight lanes a block. Bound: for
-// long rows the instructions of the rounding (2 x 131 million values in 470 us, 2.2 TB/s of f32 read), for short ones latency.
+// Rows of k and v into the cache: a warp takes up to four blocks of one row and head, eight lanes a block, keys and then values. Bound: for
+// long rows the instructions of the rounding (2 x 131 million values in 420 us, 2.5 TB/s of f32 read; keys and values by warps of their
+// own: 550), for short ones latency.
 __global__ void __launch_bounds__(256) kv4_append_kernel(Kv4 c, const float* __restrict__ k, const float* __restrict__ v, int ldkv, KvRows rows, const int* __restrict__ lens) {
     pdl_trigger();
     pdl_wait();
     const int lane = threadIdx.x & 31, seq = blockIdx.z, h = blockIdx.y, first = rows.start[seq], n = rows.start[seq + 1] - first;
     const int len = lens[seq];
     if (len < 0 || len > c.cap - n) return;
-    const long long warps = (long long)gridDim.x * (blockDim.x >> 5), parts = (c.nb + 3) / 4 * 2;
-    for (long long w = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); w < n * parts; w += warps) {
-        const int i = (int)(w / parts), part = (int)(w % parts), b = (part >> 1) * 4 + (lane >> 3), pos = len + i, e = lane & 7;
-        const bool in = b < c.nb, values = part & 1;
+    const int warps = gridDim.x * (blockDim.x >> 5), two = c.nb > 4;         // pieces a row: one, or two
+    for (int w = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); w < n << two; w += warps) {
+        const int i = w >> two, b = (w & two) * 4 + (lane >> 3), pos = len + i, e = lane & 7;
+        const bool in = b < c.nb;
         const size_t at = (size_t)(first + i) * ldkv + h * c.dim() + b * kKvBlock + 4 * e, row = c.row(seq, h, pos);
-        const float4 x = in ? *(const float4*)((values ? v : k) + at) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        const float4 none = make_float4(0.0f, 0.0f, 0.0f, 0.0f), kx = in ? *(const float4*)(k + at) : none, vx = in ? *(const float4*)(v + at) : none;
         __half d;
         int level[4];
-        quantize4(x, &d, level);
-        if (in && !e) (values ? c.vd : c.kd)[row * c.nb + b] = d;
-        if (values) {
-            const uint2 half = value_halves(level, lane);
-            if (in && e < 2) {
-                uint16_t* to = (uint16_t*)c.vq + 2 * ((row >> 1) * (c.nb * 8) + (4 * e) * c.nb + b) + (pos & 1);
-                to[0] = (uint16_t)half.x; to[2 * c.nb] = (uint16_t)(half.x >> 16);
-                to[4 * c.nb] = (uint16_t)half.y; to[6 * c.nb] = (uint16_t)(half.y >> 16);
-            }
-        } else {
-            const uint32_t word = key_word(level, lane);
-            if (in && !(e & 1)) c.kq[row * (c.nb * 4) + (e >> 1) * c.nb + b] = word;
+        quantize4(kx, &d, level);
+        const uint32_t word = key_word(level, lane);
+        if (in && !(e & 1)) c.kq[row * (c.nb * 4) + (e >> 1) * c.nb + b] = word;
+        if (in && !e) c.kd[row * c.nb + b] = d;
+        quantize4(vx, &d, level);
+        const uint2 half = value_halves(level, lane);
+        if (in && e < 2) {
+            uint16_t* to = (uint16_t*)c.vq + 2 * ((row >> 1) * (c.nb * 8) + (4 * e) * c.nb + b) + (pos & 1);
+            to[0] = (uint16_t)half.x; to[2 * c.nb] = (uint16_t)(half.x >> 16);
+            to[4 * c.nb] = (uint16_t)half.y; to[6 * c.nb] = (uint16_t)(half.y >> 16);
         }
+        if (in && !e) c.vd[row * c.nb + b] = d;
     }
 }
 
 // Positions from[seq] .. + n of every sequence as the values that they stand for: out [n_seq][n][n_kv][dim], zeros outside the cache. A thread
-// writes eight channels of a row, of keys from one word, of values from the nibble j of eight half words. Bound: the bytes written.
+// writes eight channels of a row, of keys from one word, of values from the nibble j of eight half words. Bound: the bytes written (134 MB in 27 us, 4.9 TB/s; a fill of as much
+// takes 21; 32 us without the streaming hint, 39 with each lane's 32 bytes stored by itself).
 __global__ void __launch_bounds__(256) kv4_read_kernel(Kv4 c, const int* __restrict__ from, int n, float* __restrict__ k, float* __restrict__ v) {
     pdl_trigger();
     pdl_wait();
@@ -104,7 +105,8 @@ struct __align__(16) EvictShared {
 
 // What stays of a (sequence, head), shared by gridDim.x CTAs. Each finds the key of the last position that stays for itself (three passes
 // of 11, 11 and 10 bits over the keys, in shared memory where they fit): the row of weights is short next to what is moved, and no CTA has to
-// wait for another. Then each brings a range of dst's rows. Bound: latency, and the bytes moved of long caches.
+// wait for another. Then each brings a range of dst's rows. Bound: latency, and the bytes moved of long caches (64 heads of 128, 16001 to
+// 2048 positions: 25 us, 13 of them for the move of 38 MB).
 __global__ void __launch_bounds__(ET, 1) kv4_evict_kernel(Kv4 src, Kv4 dst, const int* __restrict__ lens, int* __restrict__ lens_out, int budget, int recent,
                                                           const float* __restrict__ mass, float* __restrict__ mass_out, int* __restrict__ kept) {
     extern __shared__ __align__(16) char raw[];
@@ -274,7 +276,7 @@ __global__ void __launch_bounds__(ET, 1) kv4_evict_kernel(Kv4 src, Kv4 dst, cons
 }  // namespace
 
 int launch_kv4_append(const Kv4& c, const float* k, const float* v, int ldkv, const KvRows& rows, int max_rows, const int* lens, cudaStream_t st) {
-    const long long warps = (long long)max_rows * ((c.nb + 3) / 4) * 2;
+    const long long warps = (long long)max_rows << (c.nb > 4);
     const dim3 grid((unsigned)std::min<long long>((warps + 7) / 8, 4096), c.n_kv, c.n_seq);
     FC_CUDA(launch_pdl(kv4_append_kernel, grid, dim3(256), 0, st, c, k, v, ldkv, rows, lens));
     FC_LAUNCHED();

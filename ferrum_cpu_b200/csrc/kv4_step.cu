@@ -11,6 +11,10 @@
 // A cluster shares a (sequence, head): its warps take tiles of 32 positions in turn, each with a running maximum and sum of its
 // own and its next tiles on the way to shared memory, and join through distributed shared memory at the end: no scratch memory, nothing
 // that two calls could share, one launch. New rows go into the cache on the way, by the CTA whose tile they fall into.
+//
+// Bound: issue. A tile of heads of 128 is some 900 instructions for 4.6 KB, a third of them to form f16 levels: eight sequences of 32767
+// positions, 32 query heads on 8, take 111 us, 2.7 TB/s (47 us at the memory's rate; 141 us with the planes in products of their
+// own). 64 streams of up to 2040 positions, heads of 64, with weights: 47 us, of which uneven lengths cost a third.
 #include <cooperative_groups.h>
 
 #include "kv4_frag.cuh"

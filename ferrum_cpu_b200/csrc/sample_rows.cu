@@ -12,7 +12,8 @@
 // by chunk above those buckets, listed in them. The list gives the cut, exactly; if it does not hold the cut after all, or not all of
 // them, bisection finds it. The chunk that the random number falls into is walked by one warp.
 //
-// Bound: the instructions of the passes (a weight is 9 operations in f64 and some thirty in all), and for few rows their latency.
+// Bound: the instructions of the passes (a weight is 9 operations in f64 and some forty in all), and for few rows their latency. 192 rows of
+// 131072: 25 us for the largest, 79 for a draw without filters, 175 with top-p 0.98; a row of 32000 with all filters 19 us.
 #include <cooperative_groups.h>
 
 #include "pdl.cuh"
