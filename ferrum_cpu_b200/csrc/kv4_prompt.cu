@@ -9,11 +9,12 @@
 // the sum takes 2^-e back. Sums of products start from zero in every tile and are added to the row's in f32, because
 // the tensor core truncates.
 //
-// kv4_weights_kernel: the transposed walk. A warp keeps 32 positions' levels in registers and passes over all columns, whose
+// kv4_weights_kernel: the transposed walk. A warp keeps 32 positions' levels in registers (16 of heads
+// above 128) and passes over all columns, whose
 // maximum and sum the attention has left; each position is added up by one warp in one order.
 //
 // Bound: issue beside the products. mma.sync reaches 550 TFLOP/s alone, and 460 with three other instructions to a product; here there are
-// four to six. 6007 rows of 32 heads of 128: 2.06 ms, 144 TFLOP/s, executed twice. 2048 rows of 32 heads of 64: 147 us, their weights 102.
+// four to six. 6007 rows of 32 heads of 128: 2.06 ms, 144 TFLOP/s, executed twice. 2048 rows of 32 heads of 64: 147 us, their weights 102 (the same with 64 positions a warp).
 // One CTA of 8 warps an SM at 255 registers; two or three CTAs, or 12 warps with q in shared memory, are no faster.
 #include <cooperative_groups.h>
 
@@ -415,7 +416,7 @@ kv4_prompt_kernel(Kv4 c, Kv4Attend a, KvRows rows, int cs, float2* __restrict__ 
 constexpr int WW = 4, WCOLS = 16 * WW;           // warps; columns a pass
 template <int NB>
 struct WeightsShape {
-    static constexpr int TILES = NB <= 4 ? 4 : 2, POS = 8 * TILES * WW;       // tiles of 8 positions a warp, positions a CTA
+    static constexpr int TILES = NB <= 4 ? 4 : 2, POS = 8 * TILES * WW;      // tiles of 8 positions a warp, positions a CTA
     static constexpr int BUFS = NB <= 4 ? 2 : 1, BUF = WW * NB * 4 * 512 + WCOLS * 16, SMEM = BUFS * BUF;
 };
 
@@ -448,7 +449,7 @@ __global__ void __launch_bounds__(32 * WW) kv4_weights_kernel(Kv4 c, Kv4Attend a
     }
     float sum[TILES][2] = {};
     // the first column that sees any of the CTA's positions; the ranks take turns
-    const int col_first = max(0, j00 + 1 - base) * a.group / WCOLS * WCOLS;
+    const int col_first = min(n, max(0, j00 + 1 - base)) * a.group / WCOLS * WCOLS;
     auto from = [&](int col) {
         const int i = col / a.group, head = h * a.group + col - i * a.group;
         return col < all_cols ? a.q + (size_t)(first + i) * a.ldq + (size_t)head * DIM + 8 * t : nullptr;
@@ -547,11 +548,10 @@ __global__ void __launch_bounds__(32 * WW) kv4_weights_kernel(Kv4 c, Kv4Attend a
     cg::cluster_group cluster = cg::this_cluster();
     if (cs > 1) cluster.sync();
     else __syncthreads();
-    const int j = j00 + tid;
-    if (rank == 0 && tid < S::POS && j < end) {
+    for (int p = tid; rank == 0 && p < min(S::POS, end - j00); p += 32 * WW) {
         float x = 0.0f;
-        for (int r = 0; r < cs; ++r) x += cluster.map_shared_rank(part, r)[tid];
-        mass[j] = (j < old ? mass[j] : 0.0f) + x;
+        for (int r = 0; r < cs; ++r) x += cluster.map_shared_rank(part, r)[p];
+        mass[j00 + p] = (j00 + p < old ? mass[j00 + p] : 0.0f) + x;
     }
     if (cs > 1) cluster.sync();                  // no rank leaves while another reads its memory
 }

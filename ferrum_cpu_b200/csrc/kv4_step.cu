@@ -14,7 +14,7 @@
 //
 // Bound: issue. A tile of heads of 128 is some 900 instructions for 4.6 KB, a third of them to form f16 levels: eight sequences of 32767
 // positions, 32 query heads on 8, take 111 us, 2.7 TB/s (47 us at the memory's rate; 141 us with the planes in products of their
-// own). 64 streams of up to 2040 positions, heads of 64, with weights: 47 us, of which uneven lengths cost a third.
+// own). 64 streams of 255 to 2040 positions, heads of 64, with weights: 41 us.
 #include <cooperative_groups.h>
 
 #include "kv4_frag.cuh"
@@ -134,8 +134,26 @@ __device__ __forceinline__ uint32_t hmax2u(uint32_t a, uint32_t b) {
     return *(const uint32_t*)&r;
 }
 
+// The n-th longest sequence (the first of equals first). All threads of the CTA; s: n_seq + 1 words, free again behind the call.
+__device__ __forceinline__ int nth_longest(const int* __restrict__ lens, int n_seq, int n, int* s) {
+    const int tid = threadIdx.x;
+    static_assert(32 * SW >= kKvMaxSeq, "a thread for each sequence");
+    const int mine = tid < n_seq ? lens[tid] : 0;
+    if (tid < n_seq) s[tid] = mine;
+    __syncthreads();
+    if (tid < n_seq) {
+        int before = 0;
+        for (int q = 0; q < n_seq; ++q) before += s[q] > mine || (s[q] == mine && q < tid);
+        if (before == n) s[n_seq] = tid;
+    }
+    __syncthreads();
+    const int seq = s[n_seq];
+    __syncthreads();
+    return seq;
+}
+
 template <int NB, bool SPLIT>
-__global__ void __launch_bounds__(32 * SW, StepShape<NB>::CTAS) kv4_step_kernel(Kv4 c, Kv4Attend a, KvRows rows, float2* __restrict__ stats) {
+__global__ void __launch_bounds__(32 * SW, StepShape<NB>::CTAS) kv4_step_kernel(Kv4 c, Kv4Attend a, KvRows rows, int by_length, float2* __restrict__ stats) {
     using S = StepShape<NB>;
     constexpr int DIM = S::DIM, PAD = S::PAD, CALL = SPLIT ? COLS / 2 : COLS;      // columns of a call
     extern __shared__ __align__(16) char smem[];
@@ -145,7 +163,8 @@ __global__ void __launch_bounds__(32 * SW, StepShape<NB>::CTAS) kv4_step_kernel(
     pdl_trigger();
     pdl_wait();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const int cs = gridDim.x, rank = blockIdx.x, h = blockIdx.y % c.n_kv, col0 = blockIdx.y / c.n_kv * CALL, seq = blockIdx.z;
+    const int cs = gridDim.x, rank = blockIdx.x, h = blockIdx.y % c.n_kv, col0 = blockIdx.y / c.n_kv * CALL;
+    const int seq = by_length ? nth_longest(a.lens, c.n_seq, blockIdx.z, (int*)smem) : blockIdx.z;
     const int first = rows.start[seq], n = rows.start[seq + 1] - first, cols = min(n * a.group - col0, CALL);
     if (cols <= 0) return;                        // the whole cluster
     const int len = a.lens[seq], end = a.k ? len + n : len;
@@ -551,7 +570,10 @@ int launch_step_t(const Kv4& c, const Kv4Attend& a, const KvRows& rows, int grou
     const int most = (c.cap + TILE * SW - 1) / (TILE * SW);
     int cs = 1;
     while (cs < 8 && cs * 2 <= most && clusters * cs * 2 <= 148 * S::CTAS) cs *= 2;
-    FC_CUDA(launch_pdl_cluster(kernel, dim3(cs, c.n_kv * groups, c.n_seq), dim3(32 * SW), S::SMEM, cs, st, c, a, rows, stats));
+    // more CTAs than are resident: the long sequences go first (64 streams of 255 to 2040 positions, weights kept: 41 us, in
+    // the order of the call 47)
+    const int by_length = clusters * cs > 148 * S::CTAS && c.n_seq > 1;
+    FC_CUDA(launch_pdl_cluster(kernel, dim3(cs, c.n_kv * groups, c.n_seq), dim3(32 * SW), S::SMEM, cs, st, c, a, rows, by_length, stats));
     FC_LAUNCHED();
     return FC_OK;
 }
