@@ -12,9 +12,9 @@
 // own and its next tiles on the way to shared memory, and join through distributed shared memory at the end: no scratch memory, nothing
 // that two calls could share, one launch. New rows go into the cache on the way, by the CTA whose tile they fall into.
 //
-// Bound: issue. A tile of heads of 128 is some 900 instructions for 4.6 KB, a third of them to form f16 levels: eight sequences of 32767
-// positions, 32 query heads on 8, take 111 us, 2.7 TB/s (47 us at the memory's rate; 141 us with the planes in products of their
-// own). 64 streams of 255 to 2040 positions, heads of 64, with weights: 41 us.
+// Bound: issue. A tile of heads of 128 is 990 instructions for 4.6 KB, a third of them to form f16 levels: eight sequences of 32767
+// positions, 32 query heads on 8, take 106 us, 2.8 TB/s (47 us at the memory's rate; 141 us with the planes in products of their
+// own). 64 streams of 255 to 2040 positions, heads of 64, with weights: 40 us.
 #include <cooperative_groups.h>
 
 #include "kv4_frag.cuh"
@@ -570,7 +570,7 @@ int launch_step_t(const Kv4& c, const Kv4Attend& a, const KvRows& rows, int grou
     const int most = (c.cap + TILE * SW - 1) / (TILE * SW);
     int cs = 1;
     while (cs < 8 && cs * 2 <= most && clusters * cs * 2 <= 148 * S::CTAS) cs *= 2;
-    // more CTAs than are resident: the long sequences go first (64 streams of 255 to 2040 positions, weights kept: 41 us, in
+    // more CTAs than are resident: the long sequences go first (64 streams of 255 to 2040 positions, weights kept: 40 us, in
     // the order of the call 47)
     const int by_length = clusters * cs > 148 * S::CTAS && c.n_seq > 1;
     FC_CUDA(launch_pdl_cluster(kernel, dim3(cs, c.n_kv * groups, c.n_seq), dim3(32 * SW), S::SMEM, cs, st, c, a, rows, by_length, stats));
