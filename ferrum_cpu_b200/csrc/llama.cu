@@ -11,6 +11,7 @@
 
 #include "kv4_ops.cuh"
 #include "llama_ops.cuh"
+#include "pdl.cuh"
 
 using namespace fc;
 
@@ -419,11 +420,13 @@ int launch_attention(fc_llama_cache* s, int l, int split) {
 
 // A step that was not given up: the cache holds a position more.
 __global__ void llama_kv4_held_kernel(const StepState* st, int* held) {
+    pdl_trigger();
+    pdl_wait();
     if (!(st->done | st->error)) *held += 1;
 }
 int end_step(fc_llama_cache* s) {
     if (s->kv4.on) {
-        llama_kv4_held_kernel<<<1, 1, 0, s->m->st>>>(s->state, s->kv4.words + s->kv4.set);
+        FC_CUDA(launch_pdl(llama_kv4_held_kernel, dim3(1), dim3(1), 0, s->m->st, s->state, s->kv4.words + s->kv4.set));
         FC_LAUNCHED();
     }
     return launch_step_advance_pdl(s->state, s->m->st);

@@ -142,6 +142,8 @@ __device__ __forceinline__ void rotate_pair(float* x, int ia, int ib, float thet
 // (queries) and the n_kv heads that follow them at `k_off` are rotated in place. With `st`: the row of a decode step, at its position.
 __global__ void llama_rope_rows_kernel(float* __restrict__ qkv, int ld, int T, int n_q, int n_kv, int k_off, int hd, int half,
                                        int neox, const float2* __restrict__ ftab, float inv_linear, const StepState* st) {
+    pdl_trigger();
+    pdl_wait();
     const int r = blockIdx.x, pos = st ? st->pos : r % T;
     float* row = qkv + (size_t)r * ld;
     const int pairs = (n_q + n_kv) * half;
@@ -190,7 +192,7 @@ int launch_llama_rope_rows(float* qkv, int R, int ld, int T, int n_q, int n_kv, 
 }
 int launch_llama_rope_step(float* qkv, int n_q, int n_kv, int k_off, int hd, int rope_dim, int neox, const float2* ftab, float inv_linear, const StepState* state,
                            cudaStream_t st) {
-    llama_rope_rows_kernel<<<1, 1024, 0, st>>>(qkv, 0, 1, n_q, n_kv, k_off, hd, rope_dim / 2, neox, ftab, inv_linear, state);
+    FC_CUDA(launch_pdl(llama_rope_rows_kernel, dim3(1), dim3(1024), 0, st, qkv, 0, 1, n_q, n_kv, k_off, hd, rope_dim / 2, neox, ftab, inv_linear, state));
     FC_LAUNCHED();
     return FC_OK;
 }
