@@ -129,8 +129,13 @@ __device__ __forceinline__ uint32_t hfma2u(uint32_t a, uint32_t b, uint32_t c) {
     const __half2 r = __hfma2(*(const __half2*)&a, *(const __half2*)&b, *(const __half2*)&c);
     return *(const uint32_t*)&r;
 }
-__device__ __forceinline__ uint32_t hmax2u(uint32_t a, uint32_t b) {
-    const __half2 r = __hmax2(*(const __half2*)&a, *(const __half2*)&b);
+// a b - c
+__device__ __forceinline__ uint32_t hfms2u(uint32_t a, uint32_t b, uint32_t c) {
+    const __half2 r = __hfma2(*(const __half2*)&a, *(const __half2*)&b, __hneg2(*(const __half2*)&c));
+    return *(const uint32_t*)&r;
+}
+__device__ __forceinline__ uint32_t hmaxabs2u(uint32_t a, uint32_t b) {
+    const __half2 r = __hmax2(*(const __half2*)&a, __habs2(*(const __half2*)&b));
     return *(const uint32_t*)&r;
 }
 
@@ -224,6 +229,7 @@ __global__ void __launch_bounds__(32 * SW, StepShape<NB>::CTAS) kv4_step_kernel(
 
     // q: brought to [2^13, 2^14) by a power of two a column
     const int col = SPLIT ? g & 3 : g, plane = SPLIT ? g >> 2 : 0;
+    const uint32_t minus = plane ? 0xbc00bc00u : 0u;      // what the high plane of a weight's product is taken times in this lane
     const int c0 = SPLIT ? 2 * (t & 1) : 2 * t, c1 = c0 + 1;          // this lane's columns of scores
     Query<NB, SPLIT> q;
     {
@@ -329,7 +335,7 @@ __global__ void __launch_bounds__(32 * SW, StepShape<NB>::CTAS) kv4_step_kernel(
                 planes_of(__uint_as_float(__byte_perm(lo, hi, 0x5410)), __uint_as_float(__byte_perm(lo, hi, 0x7632)), &h0, &r0);
                 const uint32_t h1 = __shfl_xor_sync(0xffffffffu, h0, 16), r1 = __shfl_xor_sync(0xffffffffu, r0, 16);
                 ph[m][0] = plane ? h1 : h0; ph[m][1] = plane ? h0 : h1;
-                pl[m][0] = plane ? r1 : r0; pl[m][1] = plane ? r0 : r1;
+                pl[m][0] = plane ? r1 : 0u; pl[m][1] = plane ? r0 : 0u;
             } else {
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
@@ -363,10 +369,10 @@ __global__ void __launch_bounds__(32 * SW, StepShape<NB>::CTAS) kv4_step_kernel(
                     for (int b = 0; b < NB; ++b) d[m][u][b] &= sight;
                 }
 #pragma unroll
-                for (int b = 0; b < NB; ++b) most = hmax2u(most, d[m][u][b] & 0x7fff7fffu);
+                for (int b = 0; b < NB; ++b) most = hmaxabs2u(most, d[m][u][b]);
             }
-        most = hmax2u(most, __shfl_xor_sync(0xffffffffu, most, 1));
-        most = hmax2u(most, __shfl_xor_sync(0xffffffffu, most, 2));
+        most = hmaxabs2u(most, __shfl_xor_sync(0xffffffffu, most, 1));
+        most = hmaxabs2u(most, __shfl_xor_sync(0xffffffffu, most, 2));
         const int exponent = (int)(max(most & 0xffffu, most >> 16) >> 10), lift = min(15 + kScaleLift - exponent, 15);
         const uint32_t by = (uint32_t)(15 + lift) << 10;      // 2^lift, -8 <= lift
         const uint32_t up = by | by << 16;
@@ -385,8 +391,12 @@ __global__ void __launch_bounds__(32 * SW, StepShape<NB>::CTAS) kv4_step_kernel(
                 for (int u = 0; u < 2; ++u) {
                     const uint32_t f = hmul2u(d[m][u][b], up);
                     hi[u] = hmul2u(ph[m][u], f);
-                    lo[u] = hfma2u(pl[m][u], f, hfma2u(ph[m][u], f, hi[u] ^ 0x80008000u));
-                    if (SPLIT) hi[u] = plane ? lo[u] : hi[u];
+                    if (SPLIT) {
+                        // the low plane's lanes: minus the high plane, and the rest of the weight (kept for them alone)
+                        hi[u] = hfma2u(pl[m][u], f, hfma2u(ph[m][u], f, hmul2u(hi[u], minus)));
+                    } else {
+                        lo[u] = hfma2u(pl[m][u], f, hfms2u(ph[m][u], f, hi[u]));
+                    }
                 }
                 levels_of(w[2 * m][b], e0);
                 levels_of(w[2 * m + 1][b], e1);
