@@ -12,8 +12,8 @@
 // own and its next tiles on the way to shared memory, and join through distributed shared memory at the end: no scratch memory, nothing
 // that two calls could share, one launch. New rows go into the cache on the way, by the CTA whose tile they fall into.
 //
-// Bound: issue. A tile of heads of 128 is 990 instructions for 4.6 KB, a third of them to form f16 levels: eight sequences of 32767
-// positions, 32 query heads on 8, take 106 us, 2.8 TB/s (47 us at the memory's rate; 141 us with the planes in products of their
+// Bound: issue. A tile of heads of 128 is 960 instructions for 4.6 KB, a third of them to form f16 levels: eight sequences of 32767
+// positions, 32 query heads on 8, take 102 us, 3.0 TB/s (47 us at the memory's rate; 141 us with the planes in products of their
 // own). 64 streams of 255 to 2040 positions, heads of 64, with weights: 40 us.
 #include <cooperative_groups.h>
 
@@ -570,19 +570,26 @@ template <int NB, bool SPLIT>
 int launch_step_t(const Kv4& c, const Kv4Attend& a, const KvRows& rows, int groups, float2* stats, int device, cudaStream_t st) {
     using S = StepShape<NB>;
     const auto kernel = kv4_step_kernel<NB, SPLIT>;
-    static bool attr_set[64] = {};
-    if (device >= 64 || !attr_set[device]) {
+    static bool known[64] = {};
+    static int resident[64][9];                   // clusters of so many CTAs that the device holds at once
+    int here[9], *const room = device < 64 ? resident[device] : here;
+    if (device >= 64 || !known[device]) {
         FC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM));
-        if (device < 64) attr_set[device] = true;
+        for (int cs = 1; cs <= 8; ++cs) FC_CUDA(resident_clusters((const void*)kernel, dim3(32 * SW), S::SMEM, cs, &room[cs]));
+        if (device < 64) known[device] = true;
     }
-    // as many CTAs as are resident, and no more than a tile for each warp of them
+    // as many CTAs for a sequence's head as are resident together, as long as each takes tiles off the warps' shares. What is resident is asked for,
+    // not computed: clusters of 5 or 7 leave SMs of a processing cluster unused. 80 heads of 8000 positions: 3 CTAs, 40 us (2: 54), 40 heads of
+    // 32000: 6, 70 us (4: 98; 7, in two waves: 90), of 2000: 4, 10.4 us (6, with as many tiles a warp: 11.2)
     const long long clusters = (long long)c.n_seq * c.n_kv * groups;
-    const int most = (c.cap + TILE * SW - 1) / (TILE * SW);
+    const int tiles = (c.cap + TILE - 1) / TILE;
+    auto share = [&](int x) { return (tiles + SW * x - 1) / (SW * x); };
     int cs = 1;
-    while (cs < 8 && cs * 2 <= most && clusters * cs * 2 <= 148 * S::CTAS) cs *= 2;
+    for (int x = 2; x <= 8; ++x)
+        if (clusters <= room[x] && share(x) < share(cs)) cs = x;
     // more CTAs than are resident: the long sequences go first (64 streams of 255 to 2040 positions, weights kept: 40 us, in
     // the order of the call 47)
-    const int by_length = clusters * cs > 148 * S::CTAS && c.n_seq > 1;
+    const int by_length = clusters > room[cs] && c.n_seq > 1;
     FC_CUDA(launch_pdl_cluster(kernel, dim3(cs, c.n_kv * groups, c.n_seq), dim3(32 * SW), S::SMEM, cs, st, c, a, rows, by_length, stats));
     FC_LAUNCHED();
     return FC_OK;
