@@ -13,7 +13,7 @@
 // them, bisection finds it. The chunk that the random number falls into is walked by one warp.
 //
 // Bound: the instructions of the passes (a weight is 9 operations in f64 and some forty in all), and for few rows their latency. 192 rows of
-// 131072: 25 us for the largest, 79 for a draw without filters, 175 with top-p 0.98; a row of 32000 with all filters 19 us.
+// 131072: 25 us for the largest, 80 for a draw without filters, 186 with top-p 0.98, 147 with it in every other row; a row of 32000 with all filters 19 us.
 #include <cooperative_groups.h>
 
 #include "pdl.cuh"
@@ -176,13 +176,42 @@ struct Share {
     }
 };
 
+// The i-th row, of each RT rows those with top-k or top-p first (two passes more), then draws without, then the first of the largest. All
+// threads; count: RW + 1 words, free again behind the call.
+__device__ __forceinline__ int row_by_work(const fc_row_sampling* __restrict__ params, int n_rows, int V, int i, int* count) {
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, base = i - i % RT;
+    int work = -1;
+    if (base + tid < n_rows) {
+        const fc_row_sampling p = params[base + tid];
+        work = !(p.temperature > 0.0f) ? 0 : (p.top_k > 0 && p.top_k < V) || p.top_p < 1.0f ? 2 : 1;
+    }
+    const unsigned much = __ballot_sync(0xffffffffu, work == 2), some = __ballot_sync(0xffffffffu, work == 1), little = __ballot_sync(0xffffffffu, work == 0);
+    if (lane == 0) count[warp] = __popc(much) | __popc(some) << 10 | __popc(little) << 20;
+    __syncthreads();
+    int before = 0, all = 0;
+    for (int w = 0; w < RW; ++w) {
+        if (w < warp) before += count[w];
+        all += count[w];
+    }
+    const unsigned ahead = (1u << lane) - 1;
+    const int n2 = all & 1023, n1 = all >> 10 & 1023;
+    const int place = work == 2 ? (before & 1023) + __popc(much & ahead)
+                    : work == 1 ? n2 + (before >> 10 & 1023) + __popc(some & ahead) : n2 + n1 + (before >> 20) + __popc(little & ahead);
+    if (work >= 0 && place == i - base) count[RW] = base + tid;
+    __syncthreads();
+    const int row = count[RW];
+    __syncthreads();
+    return row;
+}
+
 __global__ void __launch_bounds__(RT, 4) sample_rows_kernel(const float* __restrict__ logits, long long ld, int V, const fc_row_sampling* __restrict__ params,
-                                                            const float* __restrict__ u, int* __restrict__ token, float* __restrict__ prob, int cs, int chunk, int in_shared) {
+                                                            const float* __restrict__ u, int* __restrict__ token, float* __restrict__ prob, int cs, int chunk, int in_shared, int n_rows, int by_work) {
     extern __shared__ __align__(16) char smem_raw[];
     Shared& s = *(Shared*)smem_raw;
     cg::cluster_group cluster = cg::this_cluster();
     pdl_wait();
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, rank = blockIdx.x % cs, r = blockIdx.x / cs;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, rank = blockIdx.x % cs;
+    const int r = by_work ? row_by_work(params, n_rows, V, blockIdx.x / cs, (int*)smem_raw) : blockIdx.x / cs;
     const fc_row_sampling p = params[r];
     const float* const in = logits + (size_t)r * ld;
     // whole chunks a CTA
@@ -661,8 +690,11 @@ extern "C" int fc_sample_rows_dev(int device, const float* logits, int64_t ld, i
     while ((vocab + cs - 1) / cs > chunk * (CHUNKS - 1)) chunk *= 2;
     const int share = ((vocab + cs - 1) / cs + chunk - 1) / chunk * chunk;
     const bool in_shared = share <= kSlice && (share <= kSlice / 8 || (long long)n_rows * cs <= 148);
+    // CTAs that share SMs take the rows with filters first, so that no SM has three of those and another none (192 rows of
+    // 131072, half of them with top-p: 147 us, in the order of the call 171; in a uniform batch it costs a microsecond)
+    const int by_work = n_rows > 1 && (long long)n_rows * cs > 148;
     FC_CUDA(launch_pdl_cluster(sample_rows_kernel, dim3((unsigned)n_rows * cs), dim3(RT), sizeof(Shared) + (in_shared ? (size_t)share * sizeof(float) : 0), cs, (cudaStream_t)stream,
-                               logits, (long long)ld, vocab, params, u, token, prob, cs, chunk, (int)in_shared));
+                               logits, (long long)ld, vocab, params, u, token, prob, cs, chunk, (int)in_shared, n_rows, by_work));
     FC_LAUNCHED();
     return FC_OK;
 }

@@ -201,6 +201,22 @@ def test_captured_draws_take_new_logits_and_numbers():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n", [149, 256, 257, 700])
+def test_every_row_of_a_mixed_batch_is_answered(n):
+    """Batches whose rows differ in what they take (the largest, a plain draw, filters) come back in the order of the call."""
+    rng = np.random.default_rng(n)
+    logits = (rng.standard_normal((n, 500)) * 3).astype(np.float32)
+    kinds = [(0.0, 0, 1.0, 0.0), (float("nan"), 5, 0.5, 0.0), (1.0, 0, 1.0, 0.0), (0.7, 20, 1.0, 0.0), (1.2, 0, 0.9, 0.1), (0.9, 499, 0.95, 0.0), (1.0, 500, 1.0, 0.0)]
+    params = [kinds[i] for i in rng.integers(0, len(kinds), n)]
+    u = rng.random(n).astype(np.float32)
+    token, prob = draw(logits, params, u)
+    greedy = [i for i in range(n) if not params[i][0] > 0]
+    assert (token[greedy] == logits[greedy].argmax(1)).all() and (prob[greedy] == 1).all()
+    rest = [i for i in range(n) if params[i][0] > 0]
+    check(logits[rest], [params[i] for i in rest], u[rest], token[rest], prob[rest])
+
+
+@pytest.mark.gpu
 def test_an_unknown_device_is_refused():
     z = torch.zeros(64, device="cuda")
     with pytest.raises(fcb.FerrumCudaError) as e:
