@@ -675,21 +675,29 @@ extern "C" int fc_sample_rows_dev(int device, const float* logits, int64_t ld, i
     if (!aligned16(params)) return fail(FC_E_ARG, "fc_sample_rows_dev: params must be 16-byte aligned");
     if (!n_rows) return FC_OK;
     static bool ready[64] = {};
+    static int resident[64][2][9];                // clusters of so many CTAs, with a slice in shared memory or without, that the device holds at once
+    int here[2][9], (*const room)[9] = device >= 0 && device < 64 ? resident[device] : here;
+    constexpr int kSmall = kSlice / 8;            // ids that CTAs which share an SM may hold in shared memory
     if (device < 0 || device >= 64 || !ready[device]) {
         FC_TRY(select_device(device));
         FC_CUDA(cudaFuncSetAttribute(sample_rows_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(Shared) + kSlice * sizeof(float)));
+        for (int cs = 1; cs <= 8; ++cs)
+            for (int in = 0; in < 2; ++in)
+                FC_CUDA(resident_clusters((const void*)sample_rows_kernel, dim3(RT), sizeof(Shared) + in * kSmall * sizeof(float), cs, &room[in][cs]));
         if (device < 64) ready[device] = true;
     } else {
         int current = -1;
         FC_CUDA(cudaGetDevice(&current));
         if (current != device) FC_CUDA(cudaSetDevice(device));
     }
-    // a CTA costs some microseconds whatever it holds: no more of them than are resident, 1024 ids each at least
+    // a CTA costs some microseconds whatever it holds: no more of them than are resident, 1024 ids each at least (128 rows of 131072, top-p: 4
+    // CTAs a row 126 us, 2 148; 192 rows: 2 CTAs 187 us, 3, of which not all are resident, 210)
     int cs = 1, chunk = 128;
-    while (cs < 8 && (long long)n_rows * cs * 2 <= 148 * 3 && (long long)cs * 2 * 1024 <= vocab) cs *= 2;
+    for (int x = 2; x <= 8; ++x)
+        if (n_rows <= room[vocab <= kSmall * x][x] && x * 1024 <= vocab) cs = x;
     while ((vocab + cs - 1) / cs > chunk * (CHUNKS - 1)) chunk *= 2;
     const int share = ((vocab + cs - 1) / cs + chunk - 1) / chunk * chunk;
-    const bool in_shared = share <= kSlice && (share <= kSlice / 8 || (long long)n_rows * cs <= 148);
+    const bool in_shared = share <= kSlice && (share <= kSmall || (long long)n_rows * cs <= 148);
     // CTAs that share SMs take the rows with filters first, so that no SM has three of those and another none (192 rows of
     // 131072, half of them with top-p: 147 us, in the order of the call 171; in a uniform batch it costs a microsecond)
     const int by_work = n_rows > 1 && (long long)n_rows * cs > 148;
