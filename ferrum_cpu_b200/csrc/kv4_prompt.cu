@@ -559,16 +559,21 @@ __global__ void __launch_bounds__(32 * WW) kv4_weights_kernel(Kv4 c, Kv4Attend a
 template <int NB>
 int launch_prompt_t(const Kv4& c, const Kv4Attend& a, const KvRows& rows, int max_rows, float2* stats, int device, cudaStream_t st) {
     using S = PromptShape<NB>;
-    static bool attr_set[64] = {};
-    if (device >= 64 || !attr_set[device]) {
+    static bool known[64] = {};
+    static int resident[64][9];                  // clusters of so many CTAs that the device holds at once
+    int here[9], *const room = device < 64 ? resident[device] : here;
+    if (device >= 64 || !known[device]) {
         FC_CUDA(cudaFuncSetAttribute(kv4_prompt_kernel<NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM));
-        if (device < 64) attr_set[device] = true;
+        for (int cs = 1; cs <= 8; ++cs) FC_CUDA(resident_clusters((const void*)kv4_prompt_kernel<NB>, dim3(32 * S::WARPS), S::SMEM, cs, &room[cs]));
+        if (device < 64) known[device] = true;
     }
     const long long tiles = ((long long)max_rows * a.group + S::COLS - 1) / S::COLS, ctas = tiles * c.n_kv * c.n_seq;
     if (tiles * 8 * c.n_kv > INT_MAX) return fail(FC_E_SHAPE, "%d rows of %d heads are too many for one call", max_rows, c.n_kv * a.group);
-    // a cluster shares the positions where there are fewer CTAs than the GPU holds, two tiles each at least
+    // a cluster shares the positions where there are fewer CTAs than the GPU holds, two tiles each at least (96 rows of 32 / 8 heads of 128 behind
+    // 30000 positions: 6 CTAs 400 us, 4 492)
     int cs = 1;
-    while (cs < 8 && ctas * cs * 2 <= 148 * S::CTAS && cs * 4 * KT <= c.cap) cs *= 2;
+    for (int x = 2; x <= 8; ++x)
+        if (ctas <= room[x] && x * 2 * KT <= c.cap) cs = x;
     FC_CUDA(launch_pdl_cluster(kv4_prompt_kernel<NB>, dim3((unsigned)(tiles * cs * c.n_kv), 1, c.n_seq), dim3(32 * S::WARPS), S::SMEM, cs, st, c, a, rows, cs, stats));
     FC_LAUNCHED();
     return FC_OK;
