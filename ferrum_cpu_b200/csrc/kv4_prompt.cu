@@ -569,11 +569,13 @@ int launch_prompt_t(const Kv4& c, const Kv4Attend& a, const KvRows& rows, int ma
     }
     const long long tiles = ((long long)max_rows * a.group + S::COLS - 1) / S::COLS, ctas = tiles * c.n_kv * c.n_seq;
     if (tiles * 8 * c.n_kv > INT_MAX) return fail(FC_E_SHAPE, "%d rows of %d heads are too many for one call", max_rows, c.n_kv * a.group);
-    // a cluster shares the positions where there are fewer CTAs than the GPU holds, two tiles each at least (96 rows of 32 / 8 heads of 128 behind
-    // 30000 positions: 6 CTAs 400 us, 4 492)
+    // a cluster shares the positions, two tiles of them each at least, where that shortens the rounds of CTAs; another CTA costs about two tiles (96
+    // rows of 32 / 8 heads of 128 behind 30000 positions: 6 CTAs 400 us, 4 492; 600 behind 8000, 152 tiles of columns: 704, unshared 1045).
+    // Not beyond two rounds: tiles of a prompt from its start on grow, the largest go first and the rest fill the end (2048 rows of heads of 64: 251, shared 290)
+    auto cost = [&](int x) { return (ctas + room[x] - 1) / room[x] * 840 / x * ((c.cap + KT - 1) / KT + 2 * x); };
     int cs = 1;
-    for (int x = 2; x <= 8; ++x)
-        if (ctas <= room[x] && x * 2 * KT <= c.cap) cs = x;
+    for (int x = 2; x <= 8 && ctas <= 2 * room[1]; ++x)
+        if (room[x] && x * 2 * KT <= c.cap && cost(x) < cost(cs)) cs = x;
     FC_CUDA(launch_pdl_cluster(kv4_prompt_kernel<NB>, dim3((unsigned)(tiles * cs * c.n_kv), 1, c.n_seq), dim3(32 * S::WARPS), S::SMEM, cs, st, c, a, rows, cs, stats));
     FC_LAUNCHED();
     return FC_OK;
