@@ -522,7 +522,7 @@ __global__ void __launch_bounds__(RT, 4) sample_rows_kernel(const float* __restr
                         __syncthreads();
                         n = above_n; w = above_w;
                         for (int q = 0; q < RW; ++q) { n += s.pair_n[bit & 1][q]; w += s.pair_w[bit & 1][q]; }
-                        if (enough(n, w)) { c = cand; reached = true; }
+                        if (n && enough(n, w)) { c = cand; reached = true; }      // (n: a top-p of 0 is reached ahead of the first id)
                     }
                     if (tid == 0 && reached)
                         for (int q = 0; q < cs; ++q) { *at(&s.cut, q) = c; *at(&s.found, q) = 1; }

@@ -162,6 +162,19 @@ def test_cuts_among_more_ties_than_are_listed(V, n):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("V,near,width,far", [(300, 299, 1e-3, -10.0), (2000, 500, 1e-3, -20.0), (5000, 1000, 1e-3, -20.0), (700000, 700000, 1.0, 0.0)])
+@pytest.mark.parametrize("top_p", [0.0, -1.0, 1e-30, 0.001])
+def test_a_top_p_of_next_to_nothing_leaves_the_largest(V, near, width, far, top_p):
+    """Hundreds of ids within a bucket of the largest: the cut is among them, and never above the largest."""
+    row = np.full(V, far, np.float32)
+    row[np.random.default_rng(V).permutation(V)[:near]] = np.linspace(0, width, near, dtype=np.float32)
+    rows, u = np.tile(row, (3, 1)), np.float32([0.0, 0.5, 1 - 2.0 ** -24])
+    for k in (0, 3, V // 2):
+        params = [(1.0, k, top_p, 0.0)] * 3
+        check(rows, params, u, *draw(rows, params, u))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("V", [50, 1000, 131072])
 def test_every_id_is_drawn_as_often_as_its_weight_says(V):
     """u at the middle of each of 4096 even steps: an id's count is 4096 times its probability, to a step at either end."""
