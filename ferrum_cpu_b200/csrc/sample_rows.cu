@@ -58,11 +58,12 @@ struct Row {
 };
 
 struct Weigher {
-    double scale, shift;                      // log2(e) / T; what brings the largest to 0
+    double scale, largest;                    // log2(e) / T
     float least;                              // logits below it weigh nothing (2^-45 at most): they are not asked for
     float top;                                // asked for in the place of what does not count
     const double* table;
-    __device__ __forceinline__ double log2w(float l) const { return fma((double)l, scale, shift); }
+    // the difference first (of two f32 it is next to exact): the largest is 0 whatever its size, where a rounded product of it would leave its rounding
+    __device__ __forceinline__ double log2w(float l) const { return ((double)l - largest) * scale; }
     // 2^(x + up) - z, z its table entry with the exponent, for -1000 <= x <= 0: x = (64 n + i) / 64 + r, |r| <= 1 / 128
     __device__ __forceinline__ double power(double x, int up, double* z) const {
         const double magic = 6755399441055744.0 / 64.0;      // 1.5 * 2^52 / 64: the sum's last bits are 64 x, rounded
@@ -288,9 +289,9 @@ __global__ void __launch_bounds__(RT, 4) sample_rows_kernel(const float* __restr
     if (ids.endless) { top = low = 0.0f; }
 
     const double temp = fmin(fmax((double)p.temperature, 0.01), 1e30);
-    // (45 / log2(e) = 31.2; a rounding of the product or the difference does not reach 2^-43)
+    // (45 / log2(e) = 31.2; a rounding of the difference or the product does not reach 2^-43)
     const double scale = 1.4426950408889634 / temp;
-    const Weigher weigh = {scale, -(double)top * scale, top - 31.25f * (float)temp, top, s.table};
+    const Weigher weigh = {scale, (double)top, top - 31.25f * (float)temp, top, s.table};
     const bool cut_k = p.top_k > 0 && p.top_k < V, cut_p = p.top_p < 1.0f;
     // the least logit that min-p, and 2^-40, let stay: the weight falls with the logit, so that one comparison in f32 decides
     const double floor_x = p.min_p > 0.0f ? fmax(log2(fmin((double)p.min_p, 1.0)), kLeast) : kLeast;

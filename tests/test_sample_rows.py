@@ -175,6 +175,31 @@ def test_a_top_p_of_next_to_nothing_leaves_the_largest(V, near, width, far, top_
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("V", [6, 2000, 131072])
+@pytest.mark.parametrize("size", [1e6, 1e9, 1e15, 1e16, 1e17, 1e18, 1e20, 1e24, 1e30, 1e38])
+def test_rows_of_any_size_weigh_by_differences(V, size):
+    """Ties of the largest, its neighbours, and logits a temperature or two below, at large values of either sign."""
+    rng = np.random.default_rng(V)
+    rows, params = [], []
+    for t in (1.0, 0.7, 0.01, 50.0):
+        for sign in (1, -1):
+            top = np.float32(sign * size * 1.37)
+            tied = np.full(V, top, np.float32)
+            steps = np.full(V, top, np.float32)
+            steps[rng.random(V) < 0.7] = np.nextafter(top, np.float32(-np.inf))
+            steps[V // 3] = np.nextafter(np.nextafter(top, np.float32(-np.inf)), np.float32(-np.inf))
+            below = (np.float64(top) - 3 * t * rng.random(V)).astype(np.float32)
+            far = np.full(V, -np.inf, np.float32)
+            far[[0, V - 1]] = top
+            for row in (tied, steps, below, far):
+                for k, p, m in ((0, 1.0, 0.0), (0, 0.6, 0.0), (2, 1.0, 0.0), (0, 1.0, 0.3)):
+                    rows.append(row)
+                    params.append((t, k, p, m))
+    rows, u = np.stack(rows), rng.random(len(rows)).astype(np.float32)
+    check(rows, params, u, *draw(rows, params, u))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("V", [50, 1000, 131072])
 def test_every_id_is_drawn_as_often_as_its_weight_says(V):
     """u at the middle of each of 4096 even steps: an id's count is 4096 times its probability, to a step at either end."""
