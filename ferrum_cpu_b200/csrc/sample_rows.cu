@@ -16,6 +16,8 @@
 // 131072: 25 us for the largest, 80 for a draw without filters, 186 with top-p 0.98, 147 with it in every other row; a row of 32000 with all filters 19 us.
 #include <cooperative_groups.h>
 
+#include <cfloat>
+
 #include "pdl.cuh"
 
 namespace fc {
@@ -291,12 +293,13 @@ __global__ void __launch_bounds__(RT, 4) sample_rows_kernel(const float* __restr
     const double temp = fmin(fmax((double)p.temperature, 0.01), 1e30);
     // (45 / log2(e) = 31.2; a rounding of the difference or the product does not reach 2^-43)
     const double scale = 1.4426950408889634 / temp;
-    const Weigher weigh = {scale, (double)top, top - 31.25f * (float)temp, top, s.table};
+    const Weigher weigh = {scale, (double)top, fmaxf(top - 31.25f * (float)temp, -FLT_MAX), top, s.table};
     const bool cut_k = p.top_k > 0 && p.top_k < V, cut_p = p.top_p < 1.0f;
     // the least logit that min-p, and 2^-40, let stay: the weight falls with the logit, so that one comparison in f32 decides
     const double floor_x = p.min_p > 0.0f ? fmax(log2(fmin((double)p.min_p, 1.0)), kLeast) : kLeast;
-    float keep = (float)fmax((double)top + floor_x / scale, -3.4e38);
-    for (int i = 0; i < 4 && keep > -3.4e38f && weigh.log2w(keep) >= floor_x; ++i) keep = nextafterf(keep, -INFINITY);
+    // (never above the largest, which always stays, nor below what is finite: -inf weighs nothing)
+    float keep = (float)fmax((double)top + floor_x / scale, -(double)FLT_MAX);
+    for (int i = 0; i < 4 && keep > -FLT_MAX && weigh.log2w(keep) >= floor_x; ++i) keep = nextafterf(keep, -INFINITY);
     for (int i = 0; i < 8 && keep < top && weigh.log2w(keep) < floor_x; ++i) keep = nextafterf(keep, INFINITY);
 
     u64 lane_sum = 0, warp_all = 0, lane_all = 0;

@@ -200,6 +200,27 @@ def test_rows_of_any_size_weigh_by_differences(V, size):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("V", [7, 3000, 80000])
+@pytest.mark.parametrize("forbidden", [-np.inf, np.nan])
+def test_rows_masked_with_the_lowest_value_are_drawn(V, forbidden):
+    """Every id that is left has the type's lowest value, or one next to it: finite, so that one of them is drawn."""
+    lowest, temps = np.finfo(np.float32).min, (1.0, 0.01, 1e29, 1e30)
+    rng = np.random.default_rng(V)
+    rows = np.full((5, V), lowest, np.float32)
+    rows[1, rng.random(V) < 0.5] = forbidden
+    rows[1, 3] = lowest
+    rows[2, :] = forbidden
+    rows[2, V - 1] = lowest
+    rows[3, V // 2] = np.nextafter(lowest, np.float32(0))
+    rows[4] = np.where(rng.random(V) < 0.5, lowest, np.float32(-3.4e38))
+    u = rng.random(5).astype(np.float32)
+    for t in temps:
+        for k, p, m in ((0, 1.0, 0.0), (2, 1.0, 0.0), (0, 0.5, 0.0), (0, 0.0, 0.0), (0, 1.0, 0.5), (3, 0.9, 0.1)):
+            params = [(t, k, p, m)] * 5
+            check(rows, params, u, *draw(rows, params, u))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("V", [50, 1000, 131072])
 def test_every_id_is_drawn_as_often_as_its_weight_says(V):
     """u at the middle of each of 4096 even steps: an id's count is 4096 times its probability, to a step at either end."""
