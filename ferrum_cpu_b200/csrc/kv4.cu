@@ -108,7 +108,8 @@ struct __align__(16) EvictShared {
 // wait for another. Then each brings a range of dst's rows. Bound: latency, and the bytes moved of long caches (64 heads of 128, 16001 to
 // 2048 positions: 25 us, 13 of them for the move of 38 MB).
 __global__ void __launch_bounds__(ET, 1) kv4_evict_kernel(Kv4 src, Kv4 dst, const int* __restrict__ lens, int* __restrict__ lens_out, int budget, int recent,
-                                                          const float* __restrict__ mass, float* __restrict__ mass_out, int* __restrict__ kept) {
+                                                          const float* __restrict__ mass, float* __restrict__ mass_out, int* __restrict__ kept,
+                                                          const StepState* state) {
     extern __shared__ __align__(16) char raw[];
     EvictShared& s = *(EvictShared*)raw;
     pdl_trigger();
@@ -116,6 +117,7 @@ __global__ void __launch_bounds__(ET, 1) kv4_evict_kernel(Kv4 src, Kv4 dst, cons
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, h = blockIdx.y, seq = blockIdx.z, head = seq * src.n_kv + h;
     int len = lens[seq];
     len = len < 0 ? 0 : min(len, src.cap);
+    if (state && (state->done | state->error)) budget = dst.cap;
     const int left = min(len, budget);
     if (tid == 0 && h == 0 && blockIdx.x == 0) lens_out[seq] = left;
     // this CTA's rows of dst, an even number from an even one on
@@ -296,7 +298,7 @@ int kv4_make(Arena& arena, int n_seq, int n_kv, int dim, int cap, Kv4* c) {
 }
 
 int launch_kv4_evict(const Kv4& a, const Kv4& b, const int* lens, int* lens_out, int budget, int recent, const float* mass, float* mass_out, int* kept, int device,
-                     cudaStream_t st) {
+                     cudaStream_t st, const StepState* state) {
     static bool attr_set[64] = {};
     if (device >= 64 || !attr_set[device]) {
         FC_CUDA(cudaFuncSetAttribute(kv4_evict_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(EvictShared)));
@@ -307,7 +309,7 @@ int launch_kv4_evict(const Kv4& a, const Kv4& b, const int* lens, int* lens_out,
     const long long heads = (long long)a.n_kv * a.n_seq;
     int share = 1;
     while (share < 32 && heads * share * 2 <= 148 && budget >= share * 2 * 64) share *= 2;
-    FC_CUDA(launch_pdl(kv4_evict_kernel, dim3(share, a.n_kv, a.n_seq), dim3(ET), sizeof(EvictShared), st, a, b, lens, lens_out, budget, recent, mass, mass_out, kept));
+    FC_CUDA(launch_pdl(kv4_evict_kernel, dim3(share, a.n_kv, a.n_seq), dim3(ET), sizeof(EvictShared), st, a, b, lens, lens_out, budget, recent, mass, mass_out, kept, state));
     FC_LAUNCHED();
     return FC_OK;
 }

@@ -18,8 +18,9 @@ struct Kv4Attend {
 
 // A zeroed cache in the arena's memory.
 int kv4_make(Arena& arena, int n_seq, int n_kv, int dim, int cap, Kv4* c);
+// state (may be null): with a stream that is done or in error all of it moves, into a dst of the same capacity.
 int launch_kv4_evict(const Kv4& src, const Kv4& dst, const int* lens, int* lens_out, int budget, int recent, const float* mass, float* mass_out, int* kept,
-                     int device, cudaStream_t st);
+                     int device, cudaStream_t st, const StepState* state = nullptr);
 int make_device(int device);
 int launch_kv4_append(const Kv4& c, const float* k, const float* v, int ldkv, const KvRows& rows, int max_rows, const int* lens, cudaStream_t st);
 // kv4_step.cu: few query rows a key / value head; stats: where a row's maximum (base 2) and sum go, if another kernel adds up its weights.

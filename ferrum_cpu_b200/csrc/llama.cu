@@ -70,7 +70,7 @@ struct LlamaKv4 {
     int cap = 0, budget = 0, recent = 0;
     std::vector<Kv4> layers[2];
     float* mass[2] = {nullptr, nullptr};  // [L][n_kv][cap], where positions are evicted
-    int* words = nullptr;                 // positions held by either set, 0, ids of the prompt
+    int* words = nullptr;                 // positions held by either set, 0, ids of the prompt, what a step's attention finds
     Kv4 prompt{};                         // one layer's rows of a prompt that is longer than `cap`, and their weights; made when the first comes
     float* prompt_mass = nullptr;
     int set = 0, held = 0;
@@ -406,8 +406,8 @@ int launch_attention(fc_llama_cache* s, int l, int split) {
     if (s->kv4.on) {
         const LlamaKv4& k = s->kv4;
         FC_TRY(launch_llama_rope_step(s->qkv, c.n_head, c.n_kv_head, m->q_dim, c.head_dim, c.rope_dim, c.rope_type == FC_ROPE_NEOX, m->ftab, m->inv_linear,
-                                      s->state, m->st));
-        return attend_kv4(m, k.layers[k.set][l], s->qkv, 1, k.words + k.set, k.evicts() ? k.mass[k.set] + l * kv4_layer_mass(s) : nullptr, s->att);
+                                      s->state, k.words + k.set, k.words + 4, m->st));
+        return attend_kv4(m, k.layers[k.set][l], s->qkv, 1, k.words + 4, k.evicts() ? k.mass[k.set] + l * kv4_layer_mass(s) : nullptr, s->att);
     }
     const size_t layer_stride = (size_t)c.ctx * m->kv_dim;
     float *kc = s->kc + l * layer_stride, *vc = s->vc + l * layer_stride;
@@ -574,14 +574,14 @@ void drop_graphs(fc_llama_cache* s) {
         }
 }
 
-// Room for n more positions in a 4-bit cache that evicts.
+// Room for n more positions in a 4-bit cache that evicts. Behind a step that failed nothing is evicted: the layers move whole.
 int make_room(fc_llama_cache* s, int n) {
     LlamaKv4& k = s->kv4;
     if (!k.on || !k.evicts() || k.held + n <= k.cap) return FC_OK;
     const int from = k.set, to = 1 - k.set;
     for (int l = 0; l < s->m->cfg.n_layer; ++l)
         FC_TRY(launch_kv4_evict(k.layers[from][l], k.layers[to][l], k.words + from, k.words + to, k.budget, k.recent, k.mass[from] + l * kv4_layer_mass(s),
-                                k.mass[to] + l * kv4_layer_mass(s), nullptr, s->m->device, s->m->st));
+                                k.mass[to] + l * kv4_layer_mass(s), nullptr, s->m->device, s->m->st, s->state));
     k.set = to;
     k.held = std::min(k.held, k.budget);
     return FC_OK;
@@ -663,6 +663,8 @@ int feed_ids(fc_llama_cache* s, const int32_t* ids, int n, int head_on_last) {
     if (s->host_pos + n > m->cfg.ctx)
         return fail(FC_E_DIM, "%d more tokens do not fit the model's %d-token context window (position %d)", n, m->cfg.ctx, s->host_pos);
     FC_CUDA(cudaMemcpyAsync(s->queue + s->host_pos, ids, (size_t)n * 4, cudaMemcpyHostToDevice, m->st));
+    // test hook: the last of them is lost on its way, and its step finds an id that is none
+    if (s->kv4.on && g_debug.withhold == 1) FC_CUDA(cudaMemsetAsync(s->queue + s->host_pos + n - 1, 0xff, 4, m->st));
     llama_set_state_kernel<<<1, 1, 0, m->st>>>(s->state, s->host_pos, s->host_pos, s->host_pos + n);
     FC_LAUNCHED();
     for (int i = 0; i < n; ++i) {
@@ -1005,7 +1007,7 @@ static int cache_create(fc_llama* m, const LlamaKv4* kv4, fc_llama_cache** out) 
                 for (Kv4& layer : k.layers[i]) FC_TRY(kv4_make(a, 1, c.n_kv_head, c.head_dim, k.cap, &layer));
                 if (evicts) FC_TRY(a.alloc_n(&k.mass[i], (size_t)c.n_layer * c.n_kv_head * k.cap));
             }
-            FC_TRY(a.alloc_n(&k.words, 4));
+            FC_TRY(a.alloc_n(&k.words, 5));
             k.on = true;
         } else {
             const size_t kv = (size_t)c.n_layer * c.ctx * m->kv_dim;

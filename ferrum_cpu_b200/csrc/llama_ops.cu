@@ -139,11 +139,18 @@ __device__ __forceinline__ void rotate_pair(float* x, int ia, int ib, float thet
 }
 
 // Window form: row r of the fused [R][ld] buffer sits at position r % T; its first n_q heads
-// (queries) and the n_kv heads that follow them at `k_off` are rotated in place. With `st`: the row of a decode step, at its position.
+// (queries) and the n_kv heads that follow them at `k_off` are rotated in place. With `st`: the row of a decode step, at its position; *len becomes
+// the positions *held that its attention finds, or -1, which leaves the cache alone, in a step that does nothing.
 __global__ void llama_rope_rows_kernel(float* __restrict__ qkv, int ld, int T, int n_q, int n_kv, int k_off, int hd, int half,
-                                       int neox, const float2* __restrict__ ftab, float inv_linear, const StepState* st) {
+                                       int neox, const float2* __restrict__ ftab, float inv_linear, const StepState* st,
+                                       const int* held, int* len) {
     pdl_trigger();
     pdl_wait();
+    if (st) {
+        const bool idle = st->done | st->error;
+        if (threadIdx.x == 0) *len = idle ? -1 : *held;
+        if (idle) return;
+    }
     const int r = blockIdx.x, pos = st ? st->pos : r % T;
     float* row = qkv + (size_t)r * ld;
     const int pairs = (n_q + n_kv) * half;
@@ -186,13 +193,13 @@ int launch_llama_rope_planes(const float* qkv, int R, int ld, int T, int n_q, in
 
 int launch_llama_rope_rows(float* qkv, int R, int ld, int T, int n_q, int n_kv, int k_off, int hd, int rope_dim, int neox,
                            const float2* ftab, float inv_linear, cudaStream_t st) {
-    llama_rope_rows_kernel<<<R, 256, 0, st>>>(qkv, ld, T, n_q, n_kv, k_off, hd, rope_dim / 2, neox, ftab, inv_linear, nullptr);
+    llama_rope_rows_kernel<<<R, 256, 0, st>>>(qkv, ld, T, n_q, n_kv, k_off, hd, rope_dim / 2, neox, ftab, inv_linear, nullptr, nullptr, nullptr);
     FC_LAUNCHED();
     return FC_OK;
 }
 int launch_llama_rope_step(float* qkv, int n_q, int n_kv, int k_off, int hd, int rope_dim, int neox, const float2* ftab, float inv_linear, const StepState* state,
-                           cudaStream_t st) {
-    FC_CUDA(launch_pdl(llama_rope_rows_kernel, dim3(1), dim3(1024), 0, st, qkv, 0, 1, n_q, n_kv, k_off, hd, rope_dim / 2, neox, ftab, inv_linear, state));
+                           const int* held, int* len, cudaStream_t st) {
+    FC_CUDA(launch_pdl(llama_rope_rows_kernel, dim3(1), dim3(1024), 0, st, qkv, 0, 1, n_q, n_kv, k_off, hd, rope_dim / 2, neox, ftab, inv_linear, state, held, len));
     FC_LAUNCHED();
     return FC_OK;
 }

@@ -589,6 +589,7 @@ float fc_last_score_ms(const fc_model* m);
  * made afterwards by this process and, with withhold_producers != 0, makes the producer warps of
  * those kernels copy nothing (2: their copies come, and a later exchange does not: the hidden units
  * of a decode step's block, a warp's share of a tensor-core product), so that a test can watch a wait run out and the handle stay usable.
+ * The steps of a 4-bit Llama cache wait for nothing: there the last id of a feed is lost, and its step reports FC_E_DIM.
  * Nothing faults, traps or waits without a limit. Not for production use: restore
  * (4000000000, 0) afterwards. */
 int fc_debug_set_wait_budget(long long cycles, int withhold_producers);

@@ -168,6 +168,48 @@ def test_generation_is_its_steps(layout, prec):
     m.close()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape,prec", [("llama-mini", None), ("llama-mini", _lib.FC_Q_INT8), ("llama-hd64", None)])
+def test_a_failed_step_leaves_the_cache_as_it_was(shape, prec):
+    """An id is lost on its way to a step: what the cache goes on with, evictions by received weight among it, is that of a cache
+    which never failed, to the bit. Once it fails as the cache is full, once ahead of that, and in a generation that goes on behind it."""
+    sm = synth.llama_named(shape, seed=8, perturb=True)
+    m = CudaLlama.from_synth(sm, prec=prec)
+    ids = synth.token_ids(10, 80, sm.dims["vocab"])
+    layout = dict(capacity=24, budget=12, recent=3)
+    sound, cache = m.new_cache(kv4=True, **layout), m.new_cache(kv4=True, **layout)
+    failed = lambda call: fails_without_ids(call, _lib.FC_E_DIM)  # noqa: E731
+    assert np.array_equal(m.prime(ids[:20], sound), m.prime(ids[:20], cache))
+    for i, t in enumerate(ids[20:70]):
+        if i in (2, 4, 5, 17):                                  # five to a full cache, then twelve a round
+            for _ in range(60):                                 # what one of them would add is little
+                failed(lambda: m.forward_one(ids[0], cache))
+            assert cache.pos() == 20 + i
+        assert np.array_equal(m.forward_one(t, sound), m.forward_one(t, cache)), i
+        assert cache.held() == sound.held() and cache.pos() == sound.pos()
+    # a prompt of six ids whose last is lost, and the eviction rounds of the tokens behind it
+    small = dict(capacity=8, budget=3, recent=1)
+    sound, cache = m.new_cache(kv4=True, **small), m.new_cache(kv4=True, **small)
+    failed(lambda: m.generate(ids[:6], 30, engine.sampling(temperature=0.0), cache=cache))
+    for t in ids[:5]:
+        m.forward_one(t, sound)
+    assert cache.pos() == cache.held() == 5
+    for t in ids[30:50]:
+        assert np.array_equal(m.forward_one(t, sound), m.forward_one(t, cache))
+        assert cache.held() == sound.held()
+    m.close()
+
+
+def fails_without_ids(call, code):
+    _lib.check(_lib.lib().fc_debug_set_wait_budget(200_000, 1))
+    try:
+        with pytest.raises(fcb.FerrumCudaError) as e:
+            call()
+    finally:
+        _lib.check(_lib.lib().fc_debug_set_wait_budget(4_000_000_000, 0))
+    assert e.value.code == code
+
+
 def test_layouts_are_checked_before_a_device_is_used():
     assert _lib.lib().fc_llama_cache_create_kv4(None, 0, 0, 0, C.byref(C.c_void_p())) == _lib.FC_E_ARG
     assert _lib.lib().fc_llama_cache_held(None) == 0
