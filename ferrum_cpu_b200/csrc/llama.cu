@@ -680,20 +680,10 @@ int feed_ids(fc_llama_cache* s, const int32_t* ids, int n, int head_on_last) {
 // cache rows and last-row logits to fp32 rounding (the order of the sums differs), at a fraction of
 // the launches. Short prompts keep the step path.
 constexpr int kPrimeBatchMin = 8;
-int prime_window(fc_llama_cache* s, const int32_t* ids, int n) {
+int prime_rows(fc_llama_cache* s, const int32_t* ids, int n) {
     fc_llama* m = s->m;
     const fc_llama_config& c = m->cfg;
-    if (n > c.ctx) return fail(FC_E_DIM, "%d tokens do not fit the model's %d-token context window", n, c.ctx);
     cudaStream_t st = m->st;
-    LlamaKv4& k = s->kv4;
-    if (k.on && n > k.cap && !k.prompt.kq) {
-        FC_TRY(s->arena.alloc_n(&k.prompt_mass, (size_t)c.n_kv_head * c.ctx));
-        FC_TRY(kv4_make(s->arena, 1, c.n_kv_head, c.head_dim, c.ctx, &k.prompt));
-    }
-    if (k.on) {
-        llama_set_words_kernel<<<1, 1, 0, st>>>(k.words, k.set, 0, n);
-        FC_LAUNCHED();
-    }
     m->force_fp32 = true;
     int rc = ensure_workspace(m, n);
     if (rc == FC_OK && cudaMemcpyAsync(m->ids_d, ids, (size_t)n * 4, cudaMemcpyHostToDevice, st) != cudaSuccess) rc = fail(FC_E_CUDA, "upload of the prompt failed");
@@ -709,14 +699,31 @@ int prime_window(fc_llama_cache* s, const int32_t* ids, int n) {
     else
         FC_TRY(launch_gemv_row(m->head, m->n + (size_t)(n - 1) * c.d_model, RowNorm(), nullptr, nullptr, EPI_NONE, s->logits,
                                      s->state, st));
-    FC_TRY(check_status(m));
-    s->host_pos = n;
+    return check_status(m);
+}
+int prime_window(fc_llama_cache* s, const int32_t* ids, int n) {
+    fc_llama* m = s->m;
+    const fc_llama_config& c = m->cfg;
+    if (n > c.ctx) return fail(FC_E_DIM, "%d tokens do not fit the model's %d-token context window", n, c.ctx);
+    cudaStream_t st = m->st;
+    LlamaKv4& k = s->kv4;
+    if (k.on && n > k.cap) {
+        if (!k.prompt_mass) FC_TRY(s->arena.alloc_n(&k.prompt_mass, (size_t)c.n_kv_head * c.ctx));
+        if (!k.prompt.kq) FC_TRY(kv4_make(s->arena, 1, c.n_kv_head, c.head_dim, c.ctx, &k.prompt));
+    }
     if (k.on) {
-        k.held = n <= k.cap ? n : k.budget;
-        llama_set_words_kernel<<<1, 1, 0, st>>>(k.words, k.set, k.held, 0);
+        llama_set_words_kernel<<<1, 1, 0, st>>>(k.words, k.set, 0, n);
         FC_LAUNCHED();
     }
-    return FC_OK;
+    const int rc = prime_rows(s, ids, n);
+    // a prompt that failed leaves an empty cache, also where evictions have written a length
+    if (rc == FC_OK) s->host_pos = n;
+    if (k.on) {
+        k.held = rc != FC_OK ? 0 : n <= k.cap ? n : k.budget;
+        llama_set_words_kernel<<<1, 1, 0, st>>>(k.words, k.set, k.held, 0);
+        if (rc == FC_OK) FC_LAUNCHED();          // (the first failure is the one to name)
+    }
+    return rc;
 }
 
 }  // namespace

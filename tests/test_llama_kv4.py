@@ -200,6 +200,26 @@ def test_a_failed_step_leaves_the_cache_as_it_was(shape, prec):
     m.close()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [20, 60])
+def test_a_prompt_that_fails_leaves_an_empty_cache(n):
+    """A wait of its products runs out: nothing of the prompt stays, evicted rows of one that is longer than the cache among it."""
+    sm = synth.llama_named("llama-hd64", seed=8, perturb=True)
+    m = CudaLlama.from_synth(sm)
+    ids = synth.token_ids(10, 80, sm.dims["vocab"])
+    layout = dict(capacity=24, budget=12, recent=3)
+    sound, cache = m.new_cache(kv4=True, **layout), m.new_cache(kv4=True, **layout)
+    for _ in range(2):
+        fails_without_ids(lambda: m.prime(ids[:n], cache), _lib.FC_E_TIMEOUT)
+        assert cache.pos() == cache.held() == 0
+        sound.clear()
+        for t in ids[:30]:
+            assert np.array_equal(m.forward_one(t, sound), m.forward_one(t, cache))
+            assert cache.held() == sound.held()
+    assert np.array_equal(m.prime(ids[:n], sound), m.prime(ids[:n], cache))
+    m.close()
+
+
 def fails_without_ids(call, code):
     _lib.check(_lib.lib().fc_debug_set_wait_budget(200_000, 1))
     try:
