@@ -669,10 +669,10 @@ int feed_ids(fc_llama_cache* s, const int32_t* ids, int n, int head_on_last) {
     FC_LAUNCHED();
     for (int i = 0; i < n; ++i) {
         FC_TRY(make_room(s, 1));
-        FC_TRY(run_step(s, head_on_last && i + 1 == n, s->host_pos + i));
-        s->kv4.held += 1;
+        FC_TRY(run_step(s, head_on_last && i + 1 == n, s->host_pos));
+        s->kv4.held += 1;                         // a step that cannot be launched leaves the cache at the last one that was
+        s->host_pos += 1;
     }
-    s->host_pos += n;
     return FC_OK;
 }
 

@@ -220,6 +220,36 @@ def test_a_prompt_that_fails_leaves_an_empty_cache(n):
     m.close()
 
 
+@pytest.mark.gpu
+def test_a_step_that_finds_no_memory_leaves_the_cache_at_the_last_one():
+    """Sixteen heads on one: their weights take softmax statistics, from a pool that has nothing when the last step of a feed is captured."""
+    sm = synth.SynthLlama(512, 256, 2, 16, 1, 32, 512, 128, seed=3, perturb=True)
+    m, plain = CudaLlama.from_synth(sm), Plain(sm, 12, 7, 2)
+    ids = synth.token_ids(4, 60, 512)
+    layout = dict(capacity=12, budget=7, recent=2)
+    sound, cache = m.new_cache(kv4=True, **layout), m.new_cache(kv4=True, **layout)
+    m.forward_one(ids[0], cache, want_logits=False)            # the form of a feed's first steps
+    _lib.lib().fc_debug_withhold_scratch(1)
+    try:
+        with pytest.raises(fcb.FerrumCudaError) as e:
+            m.prime(ids[:5], cache)
+        assert e.value.code == _lib.FC_E_CUDA
+        with pytest.raises(fcb.FerrumCudaError):
+            m.forward_one(ids[4], cache)
+    finally:
+        _lib.lib().fc_debug_withhold_scratch(0)
+    assert cache.pos() == cache.held() == 4
+    for t in ids[:4]:
+        m.forward_one(t, sound, want_logits=False)
+        plain.rows([t])
+    for t in ids[4:40]:
+        got = m.forward_one(t, cache)
+        assert np.array_equal(got, m.forward_one(t, sound)) and cache.held() == sound.held()
+        close(got, plain.rows([t]))
+    assert m.generate(ids[:5], 40, engine.sampling(temperature=0.0), cache=cache)[0].tolist() == m.generate(ids[:5], 40, engine.sampling(temperature=0.0), cache=sound)[0].tolist()
+    m.close()
+
+
 def fails_without_ids(call, code):
     _lib.check(_lib.lib().fc_debug_set_wait_budget(200_000, 1))
     try:
