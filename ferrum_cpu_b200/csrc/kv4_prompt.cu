@@ -155,7 +155,9 @@ __device__ __forceinline__ void tile_lay(char* buf, int tid, const RawTile<NB, P
         float d[NB], top = 0.0f;
 #pragma unroll
         for (int b = 0; b < NB; ++b) { d[b] = __half2float(r.d[b]); top = fmaxf(top, fabsf(d[b])); }
-        const int e = top > 0.0f ? (__float_as_int(top) >> 23) - 127 : 0;    // an f16 above 0 is a normal f32
+        // an f16 above 0 is a normal f32, of 2^-24 at least. Zeros bring nothing to the sums of products and must not hold the maximum that the
+        // others' planes are scaled by: seven powers of two below the least of them, which rounds a score no more than that does
+        const int e = top > 0.0f ? (__float_as_int(top) >> 23) - 127 : -31;
         const float back = exp2i(-e);
 #pragma unroll
         for (int b = 0; b < NB; ++b) ((__half*)(buf + S::VD))[b * KT + j] = __float2half_rn(d[b] * back * (float)(1 << kScaleLift));

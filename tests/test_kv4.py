@@ -412,6 +412,31 @@ def test_values_of_very_different_size_keep_their_own_precision():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("size", [1.0, 2.0 ** -8, 2.0 ** -14, 2.0 ** -19])
+@pytest.mark.parametrize("rows,heads", [(33, 4), (33, 2), (5, 4)])
+def test_values_beside_rows_of_zeros_keep_their_precision(size, rows, heads):
+    """Two positions of three hold zeros: small values of the third are as exact as large ones."""
+    rng = np.random.default_rng(11)
+    n, dim = 35, 64
+    run = Run(1, 1, dim, n)
+    k, v = draws(rng, n, dim), (size * rng.standard_normal((n, dim))).astype(np.float32)
+    v[np.arange(n) % 3 != 0] = 0.0
+    kd, vd, zero, lt = dev(k), dev(v), ints([0]), ints([n])
+    run.cache.append_dev(kd.data_ptr(), vd.data_ptr(), dim, zero.data_ptr(), rows=[n])
+    run.put(k, v, [n], [0])
+    q = draws(rng, rows, heads * dim) * np.float32(0.05)
+    qd, out = dev(q), torch.empty((rows, heads * dim), device="cuda")
+    run.cache.attend_dev(qd.data_ptr(), heads * dim, heads, lt.data_ptr(), out.data_ptr(), heads * dim, rows=[rows])
+    got = out.cpu().numpy()
+    for g in range(heads):
+        qq = q[:, g * dim:(g + 1) * dim].astype(np.float64)
+        want, _ = plain_attention(qq, run.K[0, 0, :n], run.V[0, 0, :n], [n - rows + i + 1 for i in range(rows)], 1 / math.sqrt(dim))
+        ds, top = score_error(qq, run.K[0, 0, :n], 1 / math.sqrt(dim)), np.abs(run.V[0, 0, :n]).max()
+        # as in check_attention; a score with a power of two of up to 2^5 added is rounded to 2^-20, which its weight takes times ln 2
+        assert np.abs(got[:, g * dim:(g + 1) * dim] - want).max() <= top * (2 * ds + 2 * 2.0 ** -20 + 65 * 2 * EPS)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("heads,kv,dim", [(8, 2, 64), (4, 4, 128)])
 def test_a_prompt_is_its_rows_one_by_one(heads, kv, dim):
     rng = np.random.default_rng(9)
