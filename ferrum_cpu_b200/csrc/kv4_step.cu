@@ -605,7 +605,9 @@ int launch_step_nb(const Kv4& c, const Kv4Attend& a, const KvRows& rows, int col
 }  // namespace
 
 bool kv4_step_covers(const Kv4& c, int group, int max_rows) {
-    return max_rows <= kStepRows && (long long)max_rows * group <= 64;
+    // (groups of columns and heads lie on the grid's y)
+    const long long cols = (long long)max_rows * group;
+    return max_rows <= kStepRows && cols <= 64 && c.n_kv * ((cols + COLS - 1) / COLS) <= 65535;
 }
 
 int launch_kv4_step(const Kv4& c, const Kv4Attend& a, const KvRows& rows, int max_rows, float2* stats, int device, cudaStream_t st) {

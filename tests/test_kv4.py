@@ -412,6 +412,25 @@ def test_values_of_very_different_size_keep_their_own_precision():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kv,rows", [(16384, 32), (8192, 32), (16384, 24), (65535, 3), (65535, 9)])
+@pytest.mark.parametrize("with_mass", [False, True])
+def test_heads_by_the_ten_thousand(kv, rows, with_mass):
+    rng = np.random.default_rng(13)
+    run = Run(1, kv, 32, rows + 2)
+    fill(run, rng, [2])
+    mass = rng.random((1, kv, rows + 2)).astype(np.float32) if with_mass else None
+    got, q, m = attend(run, rng, kv, [2], [rows], mass=mass)
+    some = rng.integers(0, kv, 200)                              # heads of their own: a part of them is a call of its own
+    part = Run(1, len(some), 32, rows + 2)
+    part.K, part.V = run.K[:, some], run.V[:, some]
+    pick = lambda x: x.reshape(rows, kv, 32)[:, some].reshape(rows, -1)  # noqa: E731
+    check_attention(part, len(some), [2], [rows], pick(got), pick(q), mass=mass[:, some] if with_mass else None, got_mass=m[:, some] if with_mass else None)
+    assert np.isfinite(got).all()
+    k, v = run.read()
+    assert np.array_equal(k[0, some], run.K[0, some]) and np.array_equal(v[0, some], run.V[0, some])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("size", [1.0, 2.0 ** -8, 2.0 ** -14, 2.0 ** -19])
 @pytest.mark.parametrize("rows,heads", [(33, 4), (33, 2), (5, 4)])
 def test_values_beside_rows_of_zeros_keep_their_precision(size, rows, heads):
