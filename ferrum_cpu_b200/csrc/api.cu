@@ -32,6 +32,7 @@ int fail(int code, const char* fmt, ...) {
 }
 int cuda_fail(cudaError_t e, const char* what, const char* file, int line) {
     snprintf(g_err, sizeof g_err, "CUDA error %d (%s) at %s:%d in %s", (int)e, cudaGetErrorString(e), file, line, what);
+    cudaGetLastError();           // reported here: the next call's launch must not find it
     return FC_E_CUDA;
 }
 

@@ -431,6 +431,20 @@ def test_heads_by_the_ten_thousand(kv, rows, with_mass):
 
 
 @pytest.mark.gpu
+def test_a_cache_that_finds_no_memory_fails_alone():
+    run, rng = Run(1, 2, 64, 40), np.random.default_rng(14)
+    fill(run, rng, [10])
+    for _ in range(2):
+        with pytest.raises(fcb.FerrumCudaError) as e:
+            kv4.Kv4Cache(256, 65535, 256, 1 << 24)               # some 10^17 bytes
+        assert e.value.code == _lib.FC_E_CUDA
+        got, q, _ = attend(run, rng, 4, [10], [2])
+        check_attention(run, 4, [10], [2], got, q)
+        assert np.array_equal(run.read()[0], run.K)
+        torch.zeros(8, device="cuda").add_(1)                    # nor does another library's launch
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("size", [1.0, 2.0 ** -8, 2.0 ** -14, 2.0 ** -19])
 @pytest.mark.parametrize("rows,heads", [(33, 4), (33, 2), (5, 4)])
 def test_values_beside_rows_of_zeros_keep_their_precision(size, rows, heads):
