@@ -38,6 +38,20 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
+// Pairs of f16.
+__device__ __forceinline__ uint32_t hmul2u(uint32_t a, uint32_t b) {
+    const __half2 r = __hmul2(*(const __half2*)&a, *(const __half2*)&b);
+    return *(const uint32_t*)&r;
+}
+__device__ __forceinline__ uint32_t hfma2u(uint32_t a, uint32_t b, uint32_t c) {
+    const __half2 r = __hfma2(*(const __half2*)&a, *(const __half2*)&b, *(const __half2*)&c);
+    return *(const uint32_t*)&r;
+}
+// a b - c
+__device__ __forceinline__ uint32_t hfms2u(uint32_t a, uint32_t b, uint32_t c) {
+    const __half2 r = __hfma2(*(const __half2*)&a, *(const __half2*)&b, __hneg2(*(const __half2*)&c));
+    return *(const uint32_t*)&r;
+}
 // x, y (below 2^14 in size) as two f16 planes: hi + lo holds 22 bits of each, or 2^-25 where that is more.
 __device__ __forceinline__ void planes_of(float x, float y, uint32_t* hi, uint32_t* lo) {
     const __half2 h = __floats2half2_rn(x, y);

@@ -32,7 +32,7 @@ constexpr int KT = 64;                           // positions a tile
 
 template <int NB>
 struct PromptShape {
-    static constexpr int WARPS = NB <= 4 ? 8 : 4, LAY = WARPS < 8 ? WARPS : 8;          // of which LAY lay the tiles
+    static constexpr int WARPS = NB <= 4 ? 8 : 4;
     static constexpr int COLS = 16 * WARPS, DIM = NB * kKvBlock, PAD = DIM + 4;
     static constexpr int KBYTES = NB * 4096, VBYTES = NB * 4096;                       // levels as fragments
     static constexpr int KD = KBYTES + VBYTES, VD = KD + NB * KT * 4, EX = VD + NB * KT * 2, BYTES = EX + KT * 8;   // scales; {e, 2^-e}
@@ -42,20 +42,6 @@ struct PromptShape {
     static constexpr int SMEM = QBYTES + (2 * BYTES > JOIN ? 2 * BYTES : JOIN);
     static constexpr int CTAS = 1;
 };
-
-__device__ __forceinline__ uint32_t hmul2u(uint32_t a, uint32_t b) {
-    const __half2 r = __hmul2(*(const __half2*)&a, *(const __half2*)&b);
-    return *(const uint32_t*)&r;
-}
-// a b - c
-__device__ __forceinline__ uint32_t hmsub2u(uint32_t a, uint32_t b, uint32_t c) {
-    const __half2 r = __hfma2(*(const __half2*)&a, *(const __half2*)&b, __hneg2(*(const __half2*)&c));
-    return *(const uint32_t*)&r;
-}
-__device__ __forceinline__ uint32_t hmadd2u(uint32_t a, uint32_t b, uint32_t c) {
-    const __half2 r = __hfma2(*(const __half2*)&a, *(const __half2*)&b, *(const __half2*)&c);
-    return *(const uint32_t*)&r;
-}
 
 // Channels 32 b + 8 t .. + 7 of two rows of q (rows g and g + 8 of 16), as they are; zeros for a row that is none.
 template <int NB>
@@ -169,7 +155,7 @@ template <int NB>
 __global__ void __launch_bounds__(32 * PromptShape<NB>::WARPS, PromptShape<NB>::CTAS)
 kv4_prompt_kernel(Kv4 c, Kv4Attend a, KvRows rows, int cs, float2* __restrict__ stats) {
     using S = PromptShape<NB>;
-    constexpr int WARPS = S::WARPS, DIM = S::DIM, PAD = S::PAD, THREADS = 32 * WARPS, PASS = 8 / S::LAY;
+    constexpr int WARPS = S::WARPS, DIM = S::DIM, PAD = S::PAD, THREADS = 32 * WARPS, PASS = 8 / WARPS;
     extern __shared__ __align__(16) char smem[];
     __shared__ float2 ml[S::COLS];
     pdl_trigger();
@@ -195,8 +181,7 @@ kv4_prompt_kernel(Kv4 c, Kv4Attend a, KvRows rows, int cs, float2* __restrict__ 
     char* const bufs = smem + S::QBYTES;
 
     RawTile<NB, PASS> raw;
-    const bool lays = tid < 32 * S::LAY;
-    if (lays && rank < tiles) tile_ask<NB, PASS>(c, row0 + (size_t)rank * KT, tid, raw);
+    if (rank < tiles) tile_ask<NB, PASS>(c, row0 + (size_t)rank * KT, tid, raw);
 
     const int ca = warp * 16 + g, cb = ca + 8;    // this lane's two columns
     uint32_t qh[NB][8], ql[NB][8];
@@ -226,11 +211,11 @@ kv4_prompt_kernel(Kv4 c, Kv4Attend a, KvRows rows, int cs, float2* __restrict__ 
 
     float o[NB][4][4] = {}, ma = -INFINITY, mb = -INFINITY, la = 0.0f, lb = 0.0f;
     int flip = 0;
-    if (lays && rank < tiles) tile_lay<NB, PASS>(bufs, tid, raw);
+    if (rank < tiles) tile_lay<NB, PASS>(bufs, tid, raw);
     __syncthreads();
     for (int tile = rank; tile < tiles; tile += cs) {
         const char* buf = bufs + flip * S::BYTES;
-        if (lays && tile + cs < tiles) tile_ask<NB, PASS>(c, row0 + (size_t)(tile + cs) * KT, tid, raw);
+        if (tile + cs < tiles) tile_ask<NB, PASS>(c, row0 + (size_t)(tile + cs) * KT, tid, raw);
         const int j0 = tile * KT;
         if (j0 < warp_last) {
             float s[8][4];
@@ -331,7 +316,7 @@ kv4_prompt_kernel(Kv4 c, Kv4Attend a, KvRows rows, int cs, float2* __restrict__ 
                     for (int e = 0; e < 4; ++e) {
                         const uint32_t d = e < 2 ? d0 : d1;
                         hi[e] = hmul2u(ph[k][e], d);
-                        lo[e] = hmadd2u(pl[k][e], d, hmsub2u(ph[k][e], d, hi[e]));
+                        lo[e] = hfma2u(pl[k][e], d, hfms2u(ph[k][e], d, hi[e]));
                     }
                     const uint4* vf = (const uint4*)(buf + S::KBYTES) + (b * 4 + k) * 64 + lane;
                     const uint4 v0 = vf[0], v1 = vf[32];
@@ -351,7 +336,7 @@ kv4_prompt_kernel(Kv4 c, Kv4Attend a, KvRows rows, int cs, float2* __restrict__ 
             }
         }
         flip ^= 1;
-        if (lays && tile + cs < tiles) tile_lay<NB, PASS>(bufs + flip * S::BYTES, tid, raw);
+        if (tile + cs < tiles) tile_lay<NB, PASS>(bufs + flip * S::BYTES, tid, raw);
         __syncthreads();
     }
     la += __shfl_xor_sync(0xffffffffu, la, 1);

@@ -121,19 +121,6 @@ __device__ __forceinline__ void tile_scores(const char* tile, const Query<NB, SP
     }
 }
 
-__device__ __forceinline__ uint32_t hmul2u(uint32_t a, uint32_t b) {
-    const __half2 r = __hmul2(*(const __half2*)&a, *(const __half2*)&b);
-    return *(const uint32_t*)&r;
-}
-__device__ __forceinline__ uint32_t hfma2u(uint32_t a, uint32_t b, uint32_t c) {
-    const __half2 r = __hfma2(*(const __half2*)&a, *(const __half2*)&b, *(const __half2*)&c);
-    return *(const uint32_t*)&r;
-}
-// a b - c
-__device__ __forceinline__ uint32_t hfms2u(uint32_t a, uint32_t b, uint32_t c) {
-    const __half2 r = __hfma2(*(const __half2*)&a, *(const __half2*)&b, __hneg2(*(const __half2*)&c));
-    return *(const uint32_t*)&r;
-}
 __device__ __forceinline__ uint32_t hmaxabs2u(uint32_t a, uint32_t b) {
     const __half2 r = __hmax2(*(const __half2*)&a, __habs2(*(const __half2*)&b));
     return *(const uint32_t*)&r;
