@@ -94,6 +94,8 @@ __device__ __forceinline__ unsigned weight_key(float w) {
     return w != w ? 0u : b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u);
 }
 
+// (positions above KEYS have their weights read from memory in each pass, from L2 mostly: 64 heads of 128 to 2048 positions, from 16384 25.5 us, 17500 23.5,
+// 30000 33.7)
 constexpr int ET = 1024, BINS = 2048, KEYS = 16384, LISTED = 2048;
 struct __align__(16) EvictShared {
     unsigned key[KEYS];

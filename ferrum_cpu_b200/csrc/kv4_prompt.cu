@@ -13,9 +13,12 @@
 // above 128) and passes over all columns, whose
 // maximum and sum the attention has left; each position is added up by one warp in one order.
 //
-// Bound: issue beside the products. mma.sync reaches 550 TFLOP/s alone, and 460 with three other instructions to a product; here there are
-// four to six. 6007 rows of 32 heads of 128: 2.06 ms, 144 TFLOP/s, executed twice. 2048 rows of 32 heads of 64: 147 us, their weights 102 (the same with 64 positions a warp).
-// One CTA of 8 warps an SM at 255 registers; two or three CTAs, or 12 warps with q in shared memory, are no faster.
+// Bound: the latencies of products and what depends on them, of which two warps a scheduler cover about half: 1.46 instructions a cycle, the tensor
+// pipe 53 % busy, most stalls fixed waits behind an instruction. mma.sync reaches 550 TFLOP/s alone, and 460 with three other instructions to a product;
+// here there are four to six. 6007 rows of 32 heads of 128: 2.06 ms, 144 TFLOP/s, executed twice. 2048 rows of 32 heads of 64: 146 us, their weights
+// 98 (the same with 64 positions a warp); of 128: 269 and 191.
+// One CTA of 8 warps an SM at 255 registers; two or three CTAs, or 12 warps with q in shared memory, are no faster. Heads above 128: 4 warps with q in
+// shared memory, and registers that spill (40 bytes at 160, 128 at 192, 448 at 224, 1248 at 256): 2048 rows of 32 heads of 160 493 us, of 192 603, of 256 951.
 #include <cooperative_groups.h>
 
 #include <climits>
@@ -576,7 +579,9 @@ int launch_weights_t(const Kv4& c, const Kv4Attend& a, const KvRows& rows, int m
         if (device < 64) attr_set[device] = true;
     }
     const long long tiles = (c.cap + S::POS - 1) / S::POS, ctas = tiles * c.n_kv * c.n_seq, passes = ((long long)max_rows * a.group + WCOLS - 1) / WCOLS;
-    // the first positions are seen by all columns, the last by few: a cluster shares the columns, several rounds of CTAs even out the rest
+    // the first positions are seen by all columns, the last by few: a cluster shares the columns, several rounds of CTAs even out the rest. What the
+    // cache holds is on the device: CTAs are counted for its capacity, and 2048 rows in one of 32768 (16 of 17 CTAs leave at once, clusters of 1)
+    // take 450 us for their weights where one of 2048 takes 98
     int cs = 1;
     while (cs < 8 && cs * 4 <= passes && ctas * cs < 148 * 8) cs *= 2;
     FC_CUDA(launch_pdl_cluster(kv4_weights_kernel<NB>, dim3((unsigned)(tiles * cs * c.n_kv), 1, c.n_seq), dim3(32 * WW), S::SMEM, cs, st, c, a, rows, cs, stats));

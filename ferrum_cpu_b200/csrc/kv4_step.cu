@@ -14,7 +14,9 @@
 //
 // Bound: issue. A tile of heads of 128 is 960 instructions for 4.6 KB, a third of them to form f16 levels: eight sequences of 32767
 // positions, 32 query heads on 8, take 102 us, 3.0 TB/s (47 us at the memory's rate; 141 us with the planes in products of their
-// own). 64 streams of 255 to 2040 positions, heads of 64, with weights: 40 us.
+// own). 64 streams of 255 to 2040 positions, heads of 64, with weights: 40 us. 8 sequences of 8000, 32 (64) query heads on 8: heads of 64 21 us (23), 96
+// 26 (29), 128 32 (41), 192 45 (49), 256 53 (65), half as much again with weights. Five to eight columns of heads of 128 spill 380 bytes at the 128 registers
+// of two CTAs an SM, those of 256 52 bytes.
 #include <cooperative_groups.h>
 
 #include "kv4_frag.cuh"
@@ -592,7 +594,14 @@ int launch_step_nb(const Kv4& c, const Kv4Attend& a, const KvRows& rows, int col
 }  // namespace
 
 bool kv4_step_covers(const Kv4& c, int group, int max_rows) {
-    // (groups of columns and heads lie on the grid's y)
+    // Every group of 8 columns reads the cache anew, the prompt kernel reads it once for 128. Step / prompt, us, heads on 8 (1 the last):
+    //   columns                         16         32         64
+    //   1 x 900 positions of 64      9.2 / 12.1  10.1 / 12.4  13.4 / 13.1
+    //   1 x 30000 of 64               36 / 84     38 / 86     67 / 91
+    //   16 x 2000 of 64               22 / 48     44 / 50     76 / 53
+    //   8 x 8000 of 128               71 / 204   125 / 209   240 / 220
+    //   1 x 30000 of 128, 1 head      42 / 180    43 / 182    48 / 189
+    // Only full devices lose, at 64. Groups of columns and heads lie on the grid's y.
     const long long cols = (long long)max_rows * group;
     return max_rows <= kStepRows && cols <= 64 && c.n_kv * ((cols + COLS - 1) / COLS) <= 65535;
 }

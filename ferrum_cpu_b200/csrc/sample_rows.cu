@@ -4,7 +4,7 @@
 // top_p of the whole row, min-p the logit whose weight is min_p of the largest. They therefore commute, and the row is never sorted.
 //
 // Weights are exp((l - max) / T), computed in f64 and summed as whole numbers of 2^-42: a flat row of 2^17 ids has borders 2^-17 apart, of
-// which sums in 32 bits miss one in a hundred; whole numbers can be added in any order. The exponential is Tang's (Table-driven
+// which sums in 32 bits miss one in a hundred; whole numbers can be added in any order (each is off by half of 2^-42 of the largest at most). The exponential is Tang's (Table-driven
 // implementation of the exponential function, ACM TOMS 15, 1989): 2^(i / 64) from a table, times a polynomial of degree 3, to 4e-11.
 //
 // A cluster of CTAs shares a row and passes over it two or three times: (1) the largest and the least; (2) for a top-k or top-p, counts
@@ -12,8 +12,8 @@
 // by chunk above those buckets, listed in them. The list gives the cut, exactly; if it does not hold the cut after all, or not all of
 // them, bisection finds it. The chunk that the random number falls into is walked by one warp.
 //
-// Bound: the instructions of the passes (a weight is 9 operations in f64 and some forty in all), and for few rows their latency. 192 rows of
-// 131072: 25 us for the largest, 80 for a draw without filters, 186 with top-p 0.98, 147 with it in every other row; a row of 32000 with all filters 19 us.
+// Bound: the instructions of the passes (a weight is 10 operations in f64 and some forty in all), and for few rows their latency. 192 rows of
+// 131072: 25 us for the largest, 80 for a draw without filters, 186 with top-p 0.98, 148 with it in every other row; a row of 32000 with all filters 19 us.
 #include <cooperative_groups.h>
 
 #include <cfloat>

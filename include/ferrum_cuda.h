@@ -538,9 +538,12 @@ int fc_kv4_append_dev(fc_kv4* c, const float* k, const float* v, int ldkv, const
  * 0 .. lens[s] - rows[s] + i, and a row that sees nothing is zeros.
  * mass (may be NULL) [n_seq][n_kv_head][capacity]: the weights that a position receives in this call, over the rows and the heads
  * that share it, are added to it; a position that the call brings starts from nothing.
- * Sums and statistics are held in f32 and the levels are exact: the result is that of f32 arithmetic on the cached values, bitwise
- * repeatable. Pointers 16-byte aligned, ldq, ldkv, ldo multiples of 4; out overlaps nothing else. The rows of a sequence whose
- * length is negative or whose rows do not fit are NaN, and its cache and mass are left alone. */
+ * Sums and statistics are held in f32 and the levels are exact; what they meet is held to 22 bits, or to 2^-38 of the row's largest element of q,
+ * 2^-31 of its largest weight and 2^-38 of the largest value of 32 positions where that is more. Errors are those of f32 arithmetic on the cached
+ * values (2e-7 to 5e-7), unless a head's scales lie 2^14 apart or all but 2^-8 of a row's weight lies on positions next to without values (rows
+ * of a step with 2^-16 of it beside zeros: 2e-4 of what is left). Bitwise repeatable.
+ * q, k, v and out 16-byte aligned, ldq, ldkv, ldo multiples of 4; out overlaps nothing else. The rows of a sequence whose length is negative or
+ * whose rows do not fit are NaN, and its cache and mass are left alone. */
 int fc_kv4_attend_dev(fc_kv4* c, const float* q, int ldq, int n_head, const float* k, const float* v, int ldkv, const int32_t* rows,
                       const int32_t* lens, float scale, float* mass, float* out, int ldo, void* stream);
 /* What positions from[s] .. from[s] + n - 1 of every sequence stand for (from: device [n_seq], NULL: 0): k, v [n_seq][n][n_kv_head][head_dim].
@@ -555,14 +558,15 @@ int fc_kv4_evict_dev(const fc_kv4* src, fc_kv4* dst, const int32_t* lens, int32_
                      float* mass_out, int32_t* kept, void* stream);
 
 /* The parameters of one row's draw. temperature <= 0 (or NaN): the first of the largest logits; others count as 0.01 at
- * least. top_k <= 0, top_p >= 1, min_p <= 0 (or NaN): no such filter. */
+ * least, 1e30 at most. top_k <= 0, top_p >= 1, min_p <= 0 (or NaN): no such filter. */
 typedef struct {
     float temperature;
     int32_t top_k;
     float top_p, min_p;
 } fc_row_sampling;
 /* One draw from each of n_rows rows of `vocab` logits (2^20 at most), ld floats apart, with given random numbers u [n_rows] in [0, 1).
- * w = exp((l - max) / temperature) in 64 bits. As in fc_sample_logits, all of a tie at a cut stays: ids that are not below the top_k-th
+ * w = exp((l - max) / temperature) in 64 bits, the largest being 1 whatever its size, summed as whole numbers of 2^-42. The largest always
+ * stays. As in fc_sample_logits, all of a tie at a cut stays: ids that are not below the top_k-th
  * largest logit, nor below the largest logit down to which the mass reaches top_p of the whole row; and w >= min_p. Of what
  * stays, weights under 2^-40 are nothing. The token is the first id, in index order, at which the running mass reaches u
  * times the whole; prob (may be NULL) its share of the whole. NaN logits are forbidden ids, as -inf; a row
